@@ -221,6 +221,49 @@ SIGNATURES.update({
     "awq_linear_attention_segments": (ctypes.c_int, [_vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _vp, _i64, _vp]),
 })
 
+
+def _struct(name, pointers, longs, ints, floats=()):
+    """a ctypes.Structure named after its C one: pointers, then 64-bit integers, then 32-bit ones (floats: the names of
+    those that are binary32)"""
+    fields = [(n, _vp) for n in pointers.split()] + [(n, _i64) for n in longs.split()]
+    fields += [(n, _f32 if n in floats else _i32) for n in ints.split()]
+    return type(name, (ctypes.Structure,), {"_fields_": fields, "__doc__": "the C struct of the same fields (include/awq_infer.h)"})
+
+
+# several requests at once, over a cache in 4 bits
+AwqPagePlanArgs = _struct("AwqPagePlanArgs", "cached fresh table free_pages free_in free_out lengths starts key_starts positions slots left_out",
+                          "max_tokens", "n_requests max_pages n_pages reserved")
+AwqPagedAppendArgs = _struct("AwqPagedAppendArgs", "q q_out k k_out v cosines sines positions slots cache",
+                             "ldq ldq_out ldk ldk_out ldv n_tokens max_pos", "heads kv_heads dim rot interleaved n_pages")
+AwqPagedRowsArgs = _struct("AwqPagedRowsArgs", "cache table first lengths starts k v", "ldk ldv n_rows",
+                           "n_requests max_pages n_pages kv_heads dim reserved")
+AwqPagedAttentionArgs = _struct("AwqPagedAttentionArgs", "q cache table lengths ctx workspace", "ldq ldc workspace_bytes",
+                                "n_requests max_pages n_pages heads kv_heads dim scale reserved", ("scale",))
+AwqPackedAttentionArgs = _struct("AwqPackedAttentionArgs", "q k v ctx q_starts k_starts", "ldq ldk ldv ldc n_tokens n_keys",
+                                 "n_requests heads kv_heads dim causal scale", ("scale",))
+AwqSampleArgs = _struct("AwqSampleArgs", "logits temperature top_k top_p min_p uniform ids workspace", "ld vocab n_rows workspace_bytes", "")
+
+
+class AwqRotarySpec(ctypes.Structure):
+    """struct awq_rotary_spec"""
+    _fields_ = [("kind", _i32), ("rot", _i32), ("base", ctypes.c_double), ("factor", ctypes.c_double), ("original", ctypes.c_double),
+                ("slow", ctypes.c_double), ("fast", ctypes.c_double)]
+
+
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_BANDS = range(4)
+SIGNATURES.update({
+    "awq_page_bytes": (_i64, [_i32, _i32]),
+    "awq_page_plan": (ctypes.c_int, [ctypes.POINTER(AwqPagePlanArgs), _vp]),
+    "awq_rotary_tables": (ctypes.c_int, [ctypes.POINTER(AwqRotarySpec), _i64, _vp, _vp]),
+    "awq_paged_append": (ctypes.c_int, [ctypes.POINTER(AwqPagedAppendArgs), _i32, _vp]),
+    "awq_paged_rows": (ctypes.c_int, [ctypes.POINTER(AwqPagedRowsArgs), _i32, _vp]),
+    "awq_paged_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32]),
+    "awq_paged_attention": (ctypes.c_int, [ctypes.POINTER(AwqPagedAttentionArgs), _i32, _vp]),
+    "awq_packed_attention": (ctypes.c_int, [ctypes.POINTER(AwqPackedAttentionArgs), _i32, _vp]),
+    "awq_sample_workspace_bytes": (_i64, [_i64, _i64]),
+    "awq_sample": (ctypes.c_int, [ctypes.POINTER(AwqSampleArgs), _i32, _vp]),
+})
+
 _lib = None
 
 
@@ -291,6 +334,7 @@ class AwqOpenOptions(ctypes.Structure):
 
 
 DTYPES = {None: 0, "bfloat16": 1, "float32": 2}
+DTYPE_BFLOAT16, DTYPE_FLOAT32, DTYPE_FLOAT16 = 1, 2, 3
 
 
 def open_model(model_dir, dtype=None, max_positions=0):

@@ -29,6 +29,8 @@ CONFIG_MODEL_SOURCES = ["config_model.cpp", "kugilix.cpp", "tudasun.cpp", "dense
 # the int4 model of the raw weight directory and the entry points for single kernels
 INT4_SOURCES = ["gemv.hip", "gemm.hip", "prefill.hip", "canon_prompt.hip", "attention.hip", "fused.hip", "qkv_attn.hip", "qwen3.cpp",
                 "kernel_api.cpp", "layer_api.cpp", "synth.cpp"]
+# several requests at once, over a cache in 4 bits
+BATCH_SOURCES = ["batch_api.cpp", "page_plan.hip", "paged_cache.hip", "paged_attention.hip", "packed_attention.hip", "sample.hip"]
 
 # -ffp-contract=off: every fma in the sources is written out; a contracted
 #   a*b-c*d would break bit parity with the reference's __hmul/__hsub sequence.
@@ -81,7 +83,7 @@ def build_trace_run():
 
 def build(verbose=False, oracle=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    library = CORE_SOURCES + CONFIG_MODEL_SOURCES + INT4_SOURCES
+    library = CORE_SOURCES + CONFIG_MODEL_SOURCES + INT4_SOURCES + BATCH_SOURCES
     objs = _compile(library + ["trace_run.cpp"])
     _run([hipcc, "--offload-arch=gfx950", "-shared", "-fopenmp", "-o", LIB] + [objs[s] for s in library])
     _link_trace_run(objs)

@@ -679,6 +679,190 @@ int awq_join(const awq_join_args* args, int32_t f32, void* stream);
 /* z <- a N(z) + b N(z^2) + c N(z^3) + e in place, N the division of a token's n values by their root mean square */
 int awq_polynorm(void* z, int64_t ld, int64_t n, int64_t n_tokens, const float* abce, float eps, int32_t f32, void* stream);
 
+/* ----------------------------------------------------------------------------
+ * Several requests at once, over a key/value cache held in 4 bits; no
+ * counterpart in the reference.  A step of such a batch: awq_page_plan (pages
+ * and slots of the new positions), awq_paged_append (rotary positions, keys and
+ * values into the pages), awq_packed_attention for prompts (behind
+ * awq_paged_rows where a prompt has positions in the cache already) and
+ * awq_paged_attention for single tokens, awq_sample.
+ *
+ * `dtype`: AWQ_DTYPE_BFLOAT16 or AWQ_DTYPE_FLOAT16 (awq_sample: or
+ * AWQ_DTYPE_FLOAT32).  Device pointers on the current device; 16-bit
+ * activations 16-byte aligned, their strides (in values) multiples of 8.  Nothing
+ * is allocated and the host is not waited for, so that every call may be captured.
+ *
+ * The cache is n_pages pages of 64 positions, [page][kv_head][72 * dim bytes],
+ * dim 64, 128 or 256, 16-byte aligned.  A head's part of a page: its keys [64][dim / 2 bytes], its values
+ * likewise, nibbles with the low one first; then the keys' parameters
+ * [dim / 64][scale, offset][64] in binary16, then the values'.  64 values of a
+ * position share a scale s and an offset z; nibble n stands for s n + z.  Nibble
+ * k dim / 4 + 16 g + e of a key's row is its value 64 g + 16 k + e (k < 4, e < 16),
+ * nibble c dim / 16 + 4 g + e of a value's row its value 64 g + 4 c + e (c < 16, e < 4).
+ * `table` [n_requests][max_pages] names the page of every 64 positions of a
+ * request; an entry outside 0 .. n_pages - 1 holds nothing: what it would hold is not written,
+ * not attended and read as zeros.  A slot is page * 64 + position % 64.
+ * ------------------------------------------------------------------------- */
+#define AWQ_DTYPE_FLOAT16 3 /* of these operators; awq_open does not take it */
+
+/* bytes of one page, 0 for heads that the cache does not take */
+int64_t awq_page_bytes(int32_t kv_heads, int32_t dim);
+
+/* Pages and slots of the next positions of n_requests requests (n_requests (64 max_pages + 1) and 64 n_pages below 2^31).
+ * Request i has cached[i] positions (0 .. 64 max_pages) and gets fresh[i] more (up to 64 max_pages); fresh[i] < 0: it
+ * has ended and its pages go back.  free_pages [n_pages] with *free_in entries is a
+ * list from whose end pages are taken: first the pages of ended requests are put
+ * on it in the order of the requests, then the requests take theirs in order.  A request that does not fit in max_pages is
+ * left out; one that needs pages is left out too where all that the requests up to it need together is
+ * more than there are.  A request left out keeps the positions it has, its new
+ * ones get slot -1.  Written: table (new entries), free_pages, *free_out (may be
+ * free_in), lengths [n] (positions that the requests have then; ended ones 0), starts [n + 1] and key_starts
+ * [n + 1] (sums of the fresh positions and of lengths ahead of each request; key_starts may be NULL), positions
+ * and slots of max_tokens rows (of the fresh positions one request behind the
+ * other; rows behind the last: position 0, slot -1), *left_out (requests left out, may be NULL). */
+typedef struct awq_page_plan_args {
+  const int32_t* cached;
+  const int32_t* fresh;
+  int32_t* table;
+  int32_t* free_pages;
+  const int32_t* free_in;
+  int32_t* free_out;
+  int32_t* lengths;
+  int32_t* starts;
+  int32_t* key_starts;
+  int32_t* positions;
+  int32_t* slots;
+  int32_t* left_out;
+  int64_t max_tokens;
+  int32_t n_requests, max_pages, n_pages, reserved;
+} awq_page_plan_args;
+int awq_page_plan(const awq_page_plan_args* args, void* stream);
+
+/* Rotary tables cosines and sines [max_pos][rot / 2] binary32 on the host: entry (p, i) of
+ * angle f_i p, times an amplitude.  f_i = base^(-2 i / rot), or for long contexts:
+ *   AWQ_ROTARY_LINEAR  f_i / factor: positions lie closer together
+ *   AWQ_ROTARY_BASE    the base times factor^(rot / (rot - 2)): the lowest frequency
+ *                      is divided by factor, the highest stays
+ *   AWQ_ROTARY_BANDS   f_i / factor below `slow` turns in `original` positions, f_i
+ *                      above `fast` turns, between them linearly from one to the other
+ *                      in the index at which a frequency makes so many turns; amplitude 0.1 ln(factor) + 1
+ *                      (the method of the YaRN paper, Peng et al. 2023) */
+#define AWQ_ROTARY_PLAIN 0
+#define AWQ_ROTARY_LINEAR 1
+#define AWQ_ROTARY_BASE 2
+#define AWQ_ROTARY_BANDS 3
+typedef struct awq_rotary_spec {
+  int32_t kind, rot;
+  double base, factor;           /* factor >= 1 */
+  double original, slow, fast;   /* AWQ_ROTARY_BANDS */
+} awq_rotary_spec;
+int awq_rotary_tables(const awq_rotary_spec* spec, int64_t max_pos, float* cosines, float* sines);
+
+/* Rotary positions and append.  The first `rot` values of each head of q [n_tokens][ldq]
+ * and k are turned by the row of the tables at the token's position, pairs
+ * (2 i, 2 i + 1) with interleaved != 0, (i, i + rot / 2) without, and rounded once
+ * to dtype; q_out and k_out (NULL: not written) receive the whole heads and may be q and k
+ * (with the same stride).  rot: a multiple of 16, or 0: nothing is turned.  The rounded keys and v then go into the page at the
+ * token's slot: of 64 values offset = the least, scale = (largest - least) / 15, both
+ * rounded to binary16 (values beyond its range to its largest), nibble = the nearest of 0 .. 15 to
+ * (value - offset) / scale, even ones at a tie.  64 values with a NaN or an infinity among them
+ * read as NaN.  A token with a slot outside the cache is turned only; one with a position outside 0 .. max_pos - 1
+ * is neither turned nor appended and its rows of q_out and k_out stay as they were.  Where two tokens have one slot either may be kept, in whole or
+ * in parts.  q NULL: keys and values alone; cache NULL (v, slots unused): the rotary positions alone, of k too if k is set. */
+typedef struct awq_paged_append_args {
+  const void* q;
+  void* q_out;
+  const void* k;
+  void* k_out;
+  const void* v;
+  const float* cosines;
+  const float* sines;
+  const int32_t* positions;
+  const int32_t* slots;
+  void* cache;
+  int64_t ldq, ldq_out, ldk, ldk_out, ldv, n_tokens, max_pos;
+  int32_t heads, kv_heads, dim, rot, interleaved, n_pages;
+} awq_paged_append_args;
+int awq_paged_append(const awq_paged_append_args* args, int32_t dtype, void* stream);
+
+/* Positions first[i] (NULL: 0) .. lengths[i] - 1 of every request out of the cache, as the
+ * values they stand for rounded once to dtype: row starts[i] + p - first[i] of k [n_rows][ldk] and v (either may be NULL) is
+ * position p.  Rows that no request has stay as they were. */
+typedef struct awq_paged_rows_args {
+  const void* cache;
+  const int32_t* table;
+  const int32_t* first;
+  const int32_t* lengths;
+  const int32_t* starts; /* [n_requests + 1], ascending; a request's rows end where the next one's begin */
+  void* k;
+  void* v;
+  int64_t ldk, ldv, n_rows;
+  int32_t n_requests, max_pages, n_pages, kv_heads, dim, reserved;
+} awq_paged_rows_args;
+int awq_paged_rows(const awq_paged_rows_args* args, int32_t dtype, void* stream);
+
+/* Attention of one query a request over the first lengths[i] positions of its pages
+ * (up to 64 max_pages): row i of q and ctx, head h on key/value head h / (heads / kv_heads),
+ * softmax of scale q . k, weighted sum of v.  No position: zeros.  The work is cut evenly over the chip whatever the lengths; the cut, and
+ * with it the order of a request's sums, depends on all lengths of the call.  workspace:
+ * awq_paged_workspace_bytes, 16-byte aligned, contents irrelevant; calls that share one must not overlap. */
+typedef struct awq_paged_attention_args {
+  const void* q;
+  const void* cache;
+  const int32_t* table;
+  const int32_t* lengths;
+  void* ctx;
+  void* workspace;
+  int64_t ldq, ldc, workspace_bytes;
+  int32_t n_requests, max_pages, n_pages, heads, kv_heads, dim;
+  float scale;
+  int32_t reserved;
+} awq_paged_attention_args;
+int64_t awq_paged_workspace_bytes(int32_t n_requests, int32_t heads, int32_t kv_heads, int32_t dim, int32_t max_pages);
+int awq_paged_attention(const awq_paged_attention_args* args, int32_t dtype, void* stream);
+
+/* Attention of prompts one behind the other: request i has the queries
+ * q_starts[i] .. q_starts[i + 1] - 1 and the keys k_starts[i] .. k_starts[i + 1] - 1 (k_starts NULL: as
+ * q_starts), both ascending, on the device.  causal != 0: the last query sees all keys and
+ * each query ahead of it one fewer; 0: all see all.  A query without keys: zeros.  Rows of ctx that belong to no request stay as they
+ * were.  n_tokens, n_keys: rows of q and of k and v. */
+typedef struct awq_packed_attention_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* ctx;
+  const int32_t* q_starts;
+  const int32_t* k_starts;
+  int64_t ldq, ldk, ldv, ldc, n_tokens, n_keys;
+  int32_t n_requests, heads, kv_heads, dim, causal;
+  float scale;
+} awq_packed_attention_args;
+int awq_packed_attention(const awq_packed_attention_args* args, int32_t dtype, void* stream);
+
+/* A token of each row of logits [n_rows][ld], out of `vocab` (up to 524288).  With T = temperature[row] the
+ * weight of a logit l is exp((l - largest) / T).  In the order of falling logits, lower ids first among equals, the
+ * tokens kept are those that satisfy all of
+ *   top_k[row] > 0:   the first top_k[row];
+ *   top_p[row] < 1:   the fewest whose weights sum to top_p[row] times the sum of the first top_k[row];
+ *   min_p[row] > 0:   weight >= min_p[row];
+ * the first always.  ids[row] = the first kept id, in rising order, at which the sum of the weights kept exceeds uniform[row]
+ * (in [0, 1)) times all of it.  T not above 0 (or NaN): the first token.  A NaN logit counts as -infinity; logits of +infinity share all the weight;
+ * a row without a logit above -infinity: 0.  temperature NULL: 1; top_k, top_p, min_p NULL (or an entry of top_p or min_p NaN): not limited.
+ * Weights and sums are held in 64 bits.  workspace: awq_sample_workspace_bytes, 16-byte aligned, contents irrelevant; calls that share one must not overlap. */
+typedef struct awq_sample_args {
+  const void* logits;
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  const float* uniform;
+  int32_t* ids;
+  void* workspace;
+  int64_t ld, vocab, n_rows, workspace_bytes;
+} awq_sample_args;
+int64_t awq_sample_workspace_bytes(int64_t n_rows, int64_t vocab);
+int awq_sample(const awq_sample_args* args, int32_t dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
