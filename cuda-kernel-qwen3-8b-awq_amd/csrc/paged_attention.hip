@@ -1,5 +1,6 @@
 // Attention of one query a request over a cache in 4 bits (batch.hpp).
 #include "batch.hpp"
+#include "lane_sums.hpp"
 
 namespace {
 
@@ -13,10 +14,9 @@ constexpr int kColumns = 16;  // query heads of one key/value head that share a 
 
 inline int columns_of(int group) { return std::min(group, kColumns); }
 inline int streams_of(int heads, int kv_heads) { return kv_heads * ((heads / kv_heads + kColumns - 1) / kColumns); }
-// wavefronts that share the pages of a stream (a key/value head and up to 16 of its query heads): as many as the chip holds with two
-// pages each in LDS
+// wavefronts that share the pages of a stream (a key/value head and up to 16 of its query heads): as many as the chip holds with a page each in LDS
 inline int workers_of(int n_requests, int heads, int kv_heads, int dim, int max_pages) {
-  const int64_t there = 256ll * (dim == 64 ? 16 : dim == 128 ? 8 : 4) / streams_of(heads, kv_heads);
+  const int64_t there = 256ll * (dim == 256 ? 8 : 16) / streams_of(heads, kv_heads);
   const int64_t most = (int64_t)n_requests * max_pages;
   return (int)std::max<int64_t>(kWaves, (std::min(there, most) + kWaves - 1) / kWaves * kWaves);
 }
@@ -33,14 +33,13 @@ __device__ __forceinline__ void wait_for_requests() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// sums and maxima over the four lanes with one lane % 16
-__device__ __forceinline__ float over_quarters_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, 64));
-  return fmaxf(v, __shfl_xor(v, 32, 64));
-}
-__device__ __forceinline__ float over_quarters_sum(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+// over the lanes of one head: those 16 apart and, where FROM < 16, those FROM, 2 FROM .. apart too
+template <int FROM, typename F>
+__device__ __forceinline__ float over_head(float v, F f) {
+  if constexpr (FROM <= 4) v = f(v, lanes::from<0x124>(v));  // rotated by 4 within 16 lanes, and by 8
+  if constexpr (FROM <= 8) v = f(v, lanes::from<0x128>(v));
+  v = f(v, __shfl_xor(v, 16, 64));
+  return f(v, __shfl_xor(v, 32, 64));
 }
 
 __device__ __forceinline__ int pages_of(const awq_paged_attention_args& a, int r) {
@@ -60,38 +59,49 @@ __device__ __forceinline__ int pages_ahead(const awq_paged_attention_args& a, in
   all = __builtin_amdgcn_readlane(sum, 63);
   return sum - mine;
 }
-__device__ __forceinline__ int first_page(int64_t worker, int all, int workers) { return (int)(worker * all / workers); }
+// pages of a worker: equal runs, the last ones may be without
+__device__ __forceinline__ int run_of(int all, int workers) { return (all + workers - 1) / workers; }
 
 // The pages of all requests in a row are cut evenly over `workers` wavefronts; a worker walks the requests that its run touches.  A page
-// comes into LDS as it lies in memory but for the order of its 16-byte pieces, the next one while this one is worked on.  Operands of
-// v_mfma_f32_16x16x32_f16, lane (m, kg) = (lane % 16, lane / 16), heads as columns:
+// comes into LDS as it lies in memory but for the order of its 16-byte pieces, the next one's keys while this one's values are worked on and
+// the other way round.  Operands of v_mfma_f32_16x16x32_f16, lane (m, kg) = (lane % 16, lane / 16), heads as columns:
 //     S[key][head] = K q^T        sixteen keys; a lane takes quarter kg of key m's row
 //     O[c][head] += V^T P         two of sixteen keys; a lane takes piece m of the rows of the keys 4 kg .. + 3 of both
-// so that the weights a lane forms are the elements it supplies to the second product.  Nibbles go into the products as they are: as the last
+// so that the weights a lane forms are the elements it supplies to the second product.  With COLUMNS heads below 16 the columns are the heads
+// once for each of TP = 16 / COLUMNS sixteens of keys: a lane keeps the scores of its own sixteen (of every TP), supplies zeros to the
+// second product for the others, and the columns of a head are added up at the end.  Softmax is then a quarter of the instructions at 4 heads.
+// Nibbles go into the products as they are: as the last
 // bits of a binary16 number they stand for n 2^-24, four bits up for 16 times that (the query's values there are divided by 16, and
 // so are the sums of the values' pieces), so that a word of eight takes five instructions.  The scales are put on afterwards: on a key's
 // sum over a group, s sum(q n) + z sum(q) in binary32, and on the weights, p s rounded to binary16 for the product, p z in binary32.
 // Weights are relative to the largest of score + exponent of the page's largest value scale, so that p s is below 1 and as exact as
 // binary16 can be whatever the values' size.
-template <typename T, int D>
-__global__ __launch_bounds__(64 * kWaves) void paged_kernel(PagedArgs p) {
+template <typename T, int D, int COLUMNS>
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 4) void paged_kernel(PagedArgs p) {
   constexpr int G = D / 64, PIECES = D / 32;  // groups; 16-byte pieces of a row
-  constexpr int kBytes = 72 * D, kLoads = (kBytes / 16 + 63) / 64;
+  constexpr int TP = 16 / COLUMNS, SETS = 4 / TP;
+  constexpr int kBytes = 72 * D, kKeyLoads = D / 32 + (D + 127) / 128, kValueLoads = D / 32;
   typedef __attribute__((address_space(1))) const void* gptr_t;
   typedef __attribute__((address_space(3))) void* lptr_t;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves * 2 * kBytes];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves * kBytes];
   const awq_paged_attention_args& a = p.a;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, kg = lane >> 4;
   const int stream = blockIdx.x % p.streams, worker = blockIdx.x / p.streams * kWaves + wave;
   const int tiles = p.streams / a.kv_heads, kv_head = stream / tiles, group = a.heads / a.kv_heads;
   const int head0 = kv_head * group + stream % tiles * kColumns, columns = min(kColumns, group - stream % tiles * kColumns);
-  uint8_t* const mine = lds + wave * 2 * kBytes;
+  const int column = m % COLUMNS, mine = m / COLUMNS;  // which sixteen of every TP
+  // a page's keys, its parameters, its values
+  uint8_t* const kb = lds + wave * kBytes;
+  uint8_t* const pb = kb + 32 * D;
+  uint8_t* const vb = pb + 8 * D;
 
   const int run = (a.n_requests + 63) / 64;
   int all;
   const int ahead = pages_ahead(a, lane, run, all);
-  const int begin = first_page(worker, all, p.workers), end = first_page(worker + 1, all, p.workers);
-  if (begin >= end) return;
+  const int each = run_of(all, p.workers), begin = worker * each, end = min(begin + each, all);
+  if (begin >= all) return;
+  // pages of the four workers side by side, where all have some
+  const int wg_begin = (worker - wave) * each, wg_end = wg_begin + 3 * each < all ? min(wg_begin + kWaves * each, all) : INT32_MAX;
   // the request of the first page: the last run of requests that does not start behind it, then one after the other
   const int at = 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(ahead <= begin));
   int r = at * run, start = __builtin_amdgcn_readlane(ahead, at), n_pages = pages_of(a, r);
@@ -100,26 +110,47 @@ __global__ __launch_bounds__(64 * kWaves) void paged_kernel(PagedArgs p) {
     n_pages = pages_of(a, ++r);
   }
 
-  // where the lane's 16 bytes of a request into LDS come from: a key's pieces rotated among its row's, so that those that lanes read together
-  // lie in all banks; rows of values with those four apart side by side
-  const auto piece_at = [&](int i) __attribute__((always_inline)) {
-    const int x = 64 * i + lane;
-    if (x < 64 * PIECES) {
-      const int row = x / PIECES, part = x % PIECES;
-      return row * PIECES + (part ^ ((row * PIECES / 16) & (PIECES - 1)));
-    }
-    if (x < 128 * PIECES) {
-      const int slot = x / PIECES - 64, part = x % PIECES;
-      return (64 + (slot & ~15) + (slot & 3) * 4 + ((slot & 15) >> 2)) * PIECES + part;
-    }
-    return x;
+  // Where the lane's 16 bytes of a request into LDS come from: a key's pieces rotated among its row's, so that those that lanes read together
+  // lie in all banks; rows of values with those four apart side by side.  A place of the wavefront and one of the lane, which is the same in every
+  // request (of rows of 128 bytes a rotation by four pieces in every other).
+  const uint32_t key_row = lane / PIECES, in_row = lane % PIECES;
+  const uint32_t key_lane = (key_row * PIECES + (in_row ^ ((key_row * PIECES / 16) & (PIECES - 1)))) * 16;
+  const uint32_t value_slot = lane / PIECES;
+  const uint32_t value_lane = (((value_slot & ~15u) + (value_slot & 3) * 4 + ((value_slot & 15) >> 2)) * PIECES + in_row) * 16;
+  const uint32_t parameter_lane = lane * 16;
+  // (nothing of the compiler's may change the order of the requests: they are waited for by their number)
+  const auto in_order = []() __attribute__((always_inline)) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
   };
-  const auto request = [&](int page, int buffer) __attribute__((always_inline)) {
-    const uint8_t* const src = (const uint8_t*)a.cache + ((int64_t)page * a.kv_heads + kv_head) * kBytes;
+  const auto page_of = [&](int page) __attribute__((always_inline)) {
+    return (const uint8_t*)a.cache + ((int64_t)__builtin_amdgcn_readfirstlane(page) * a.kv_heads + kv_head) * kBytes;
+  };
+  // (the wavefront's place stays in scalar registers, out of the compiler's hands: it would make 64-bit addresses of each lane's)
+  const auto request = [&](const uint8_t* src, uint32_t of_lane, uint8_t* to) __attribute__((always_inline)) {
+    uint64_t place = (uint64_t)src;
+    asm volatile("" : "+s"(place));
+    __builtin_amdgcn_global_load_lds((gptr_t)(place + of_lane), (lptr_t)to, 16, 0, 0);
+  };
+  const auto request_keys = [&](int page) __attribute__((always_inline)) {
+    const uint8_t* const src = page_of(page);
+    in_order();
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-      if (64 * (i + 1) <= kBytes / 16 || lane < kBytes / 16 - 64 * i)
-        __builtin_amdgcn_global_load_lds((gptr_t)(src + piece_at(i) * 16), (lptr_t)(mine + buffer * kBytes + i * 1024), 16, 0, 0);
+    for (int i = 0; i < D / 32; ++i)
+      request(src + i * 1024, D == 256 && i % 2 ? key_lane ^ 64u : key_lane, kb + i * 1024);
+#pragma unroll
+    for (int i = 0; i < (D + 127) / 128; ++i)
+      if (D != 64 || lane < 32)
+        request(src + 64 * D + i * 1024, parameter_lane, pb + i * 1024);
+    in_order();
+  };
+  const auto request_values = [&](int page) __attribute__((always_inline)) {
+    const uint8_t* const src = page_of(page);
+    in_order();
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+      request(src + 32 * D + (D == 256 ? (i / 2) * 2048 + (i % 2) * 256 : i * 1024), value_lane, vb + i * 1024);
+    in_order();
   };
 
   for (int at_page = begin; at_page < end; ++r) {
@@ -129,27 +160,46 @@ __global__ __launch_bounds__(64 * kWaves) void paged_kernel(PagedArgs p) {
     if (n_pages == 0) continue;
     const int from = at_page - start, to = min(n_pages, end - start);
     const int32_t* const table = a.table + (int64_t)r * a.max_pages;
-
-    // the query: lane (m, kg) has values 64 g + 16 kg + 8 j .. + 7 of head m
-    half8_t qop[2 * G];
-    float q_sum[G], q_max = 0.0f;
-    {
-      float qv[2 * G][8];
-      const T* const q = (const T*)a.q + (int64_t)r * a.ldq + (int64_t)(head0 + m) * D + 16 * kg;
-      typedef T eight_t __attribute__((ext_vector_type(8)));
-#pragma unroll
-      for (int i = 0; i < 2 * G; ++i) {
-        eight_t x;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = (T)0.0f;
-        if (m < columns) x = *reinterpret_cast<const eight_t*>(q + 64 * (i / 2) + 8 * (i % 2));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          qv[i][e] = (float)x[e];
-          q_max = fmaxf(q_max, fabsf(qv[i][e]));
-        }
+    int entries = -1, entries_at = -64;
+    const auto page_at = [&](int i) __attribute__((always_inline)) {
+      if (i >= entries_at + 64) {
+        entries_at = i;
+        entries = i + lane < n_pages ? table[i + lane] : -1;
+        // (waited for here: behind the branch the wait would be one for the pages on their way too, every time)
+        asm volatile("" : "+v"(entries));
       }
-      q_max = over_quarters_max(q_max);
+      return held_page(__builtin_amdgcn_readlane(entries, i - entries_at), a.n_pages);
+    };
+
+    // the query: lane (m, kg) has values 64 g + 16 kg + 8 j .. + 7 of its head
+    typedef T eight_t __attribute__((ext_vector_type(8)));
+    eight_t qv[2 * G];
+    {
+      const T* const q = (const T*)a.q + (int64_t)r * a.ldq + (int64_t)(head0 + min(column, columns - 1)) * D + 16 * kg;
+#pragma unroll
+      for (int i = 0; i < 2 * G; ++i) qv[i] = *reinterpret_cast<const eight_t*>(q + 64 * (i / 2) + 8 * (i % 2));
+    }
+    int i = from;
+    // (an entry that is no page is passed over)
+    const auto next_page = [&]() __attribute__((always_inline)) {
+      int page = -1;
+      while (i < to && (page = page_at(i)) < 0) ++i;
+      return page;
+    };
+    int here = next_page();
+    if (here >= 0) {
+      request_keys(here);
+      request_values(here);
+    }
+    half8_t qop[2 * G];
+    float q_sum[G], mul;
+    {
+      float q_max = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2 * G; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q_max = fmaxf(q_max, fabsf((float)qv[i][e]));
+      q_max = over_head<16>(q_max, lanes::Max());
       // a power of two brings the largest to 2^14: nothing is lost of what is within 2^-24 of it
       int e2 = 0;
       if (q_max > 0.0f && q_max < INFINITY) e2 = 15 - __builtin_amdgcn_frexp_expf(q_max);
@@ -162,17 +212,16 @@ __global__ __launch_bounds__(64 * kWaves) void paged_kernel(PagedArgs p) {
           float v[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            v[e] = qv[2 * g + j][e] * up * more;
+            v[e] = (float)qv[2 * g + j][e] * up * more;
             q_sum[g] += v[e];
           }
           qop[2 * g + j] = half8_t{(half_t)v[0], (half_t)v[4], (half_t)(v[1] * 0.0625f), (half_t)(v[5] * 0.0625f),
                                    (half_t)v[2], (half_t)v[6], (half_t)(v[3] * 0.0625f), (half_t)(v[7] * 0.0625f)};
         }
-        q_sum[g] = over_quarters_sum(q_sum[g]);
+        q_sum[g] = over_head<16>(q_sum[g], lanes::Add()) * 0x1p-24f;
       }
-      q_max = __builtin_amdgcn_ldexpf(a.scale * 1.44269504088896340736f, -e2);
+      mul = __builtin_amdgcn_ldexpf(a.scale * 1.44269504088896340736f, 24 - e2);
     }
-    const float mul = q_max;
 
     f32x4_t o[G][4];
     float off[G], best = -INFINITY, sum = 0.0f;
@@ -182,37 +231,13 @@ __global__ __launch_bounds__(64 * kWaves) void paged_kernel(PagedArgs p) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[g][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    int entries = -1, entries_at = -64;
-    const auto page_at = [&](int i) __attribute__((always_inline)) {
-      if (i >= entries_at + 64) {
-        entries_at = i;
-        entries = i + lane < n_pages ? table[i + lane] : -1;
-        // (waited for here: behind the branch the wait would be one for the pages on their way too, every time)
-        asm volatile("" : "+v"(entries));
-      }
-      return held_page(__builtin_amdgcn_readlane(entries, i - entries_at), a.n_pages);
-    };
-    int page = page_at(from);
-    if (page >= 0) request(page, 0);
-    for (int i = from; i < to; ++i) {
-      const int buffer = (i - from) & 1;
-      const int next = i + 1 < to ? page_at(i + 1) : -1;
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the other buffer has been read
-      if (next >= 0) {
-        request(next, buffer ^ 1);
-        wait_for_requests<kLoads>();
-      } else {
-        wait_for_requests<0>();
-      }
-      const int here = page;
-      page = next;
-      if (here < 0) continue;
-      const uint8_t* const kb = mine + buffer * kBytes;
-      const uint8_t* const vb = kb + 32 * D;
+    while (here >= 0) {
       const int left = length - i * kPage;  // positions of this page
-
-      float score[4][4];
-      float highest = -INFINITY;
+      ++i;
+      const int next = next_page();
+      // requests on their way: this page's keys and parameters, then its values
+      wait_for_requests<kValueLoads>();
+      f32x4_t s[SETS][G];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const int row = 16 * t + m, turn = (row * PIECES / 16) & (PIECES - 1);
@@ -228,51 +253,65 @@ __global__ __launch_bounds__(64 * kWaves) void paged_kernel(PagedArgs p) {
             for (int e = 0; e < 4; ++e) w[4 * i4 + e] = x[e];
           }
         }
-        f32x4_t s[G];
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          s[g] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+          f32x4_t one = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const uint32_t x = w[2 * g + j], y = x >> 8;
             const u32x4_t op = u32x4_t{x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u};
-            s[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, op), qop[2 * g + j], s[g], 0, 0, 0);
+            one = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, op), qop[2 * g + j], one, 0, 0, 0);
           }
-        }
+          if (t % TP == 0) s[t / TP][g] = one;
+          else
 #pragma unroll
-        for (int e = 0; e < 4; ++e) score[t][e] = 0.0f;
+            for (int e = 0; e < 4; ++e) s[t / TP][g][e] = mine == t % TP ? one[e] : s[t / TP][g][e];
+        }
+      }
+      float score[SETS][4], highest = -INFINITY;
+#pragma unroll
+      for (int q = 0; q < SETS; ++q) {
+        const int row = 16 * (q * TP + mine) + 4 * kg;  // of the lane's four keys
+#pragma unroll
+        for (int e = 0; e < 4; ++e) score[q][e] = 0.0f;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          const half4_t sc = *reinterpret_cast<const half4_t*>(kb + page_parameter(D, 0, g, 0, 16 * t + 4 * kg));
-          const half4_t zz = *reinterpret_cast<const half4_t*>(kb + page_parameter(D, 0, g, 1, 16 * t + 4 * kg));
+          const half4_t sc = *reinterpret_cast<const half4_t*>(pb + ((g * 2) * kPage + row) * 2);
+          const half4_t zz = *reinterpret_cast<const half4_t*>(pb + ((g * 2 + 1) * kPage + row) * 2);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            score[t][e] = __builtin_fmaf((float)sc[e], s[g][e] * 0x1p24f, __builtin_fmaf((float)zz[e], q_sum[g], score[t][e]));
+            score[q][e] = __builtin_fmaf((float)sc[e], s[q][g][e], __builtin_fmaf((float)zz[e], q_sum[g], score[q][e]));
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          score[t][e] = 16 * t + 4 * kg + e < left ? score[t][e] * mul : -INFINITY;
-          highest = fmaxf(highest, score[t][e]);
+          score[q][e] = row + e < left ? score[q][e] * mul : -INFINITY;
+          highest = fmaxf(highest, score[q][e]);
         }
       }
-      half4_t vs[G][4], vz[G][4];
-      float widest = 0.0f;
+      half4_t vs[SETS][G], vz[SETS][G];
+      half4_t widest4 = half4_t{};
 #pragma unroll
-      for (int g = 0; g < G; ++g)
+      for (int q = 0; q < SETS; ++q) {
+        const int row = 16 * (q * TP + mine) + 4 * kg;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          vs[g][t] = *reinterpret_cast<const half4_t*>(kb + page_parameter(D, 1, g, 0, 16 * t + 4 * kg));
-          vz[g][t] = *reinterpret_cast<const half4_t*>(kb + page_parameter(D, 1, g, 1, 16 * t + 4 * kg));
-          if (left < kPage) {  // whatever lies behind the last position
+        for (int g = 0; g < G; ++g) {
+          vs[q][g] = *reinterpret_cast<const half4_t*>(pb + 4 * D + ((g * 2) * kPage + row) * 2);
+          vz[q][g] = *reinterpret_cast<const half4_t*>(pb + 4 * D + ((g * 2 + 1) * kPage + row) * 2);
+        }
+        if (left < kPage) {  // whatever lies behind the last position
+#pragma unroll
+          for (int g = 0; g < G; ++g)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (16 * t + 4 * kg + e >= left) vs[g][t][e] = vz[g][t][e] = (half_t)0.0f;
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) widest = fmaxf(widest, (float)vs[g][t][e]);
+              if (row + e >= left) vs[q][g][e] = vz[q][g][e] = (half_t)0.0f;
         }
-      highest = over_quarters_max(highest);
-      widest = over_quarters_max(widest);
+#pragma unroll
+        for (int g = 0; g < G; ++g) widest4 = __builtin_elementwise_max(widest4, vs[q][g]);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the keys and the parameters have been read
+      if (next >= 0) request_keys(next);
+      highest = over_head<COLUMNS>(highest, lanes::Max());
+      const float widest = over_head<COLUMNS>(fmaxf(fmaxf((float)widest4[0], (float)widest4[1]), fmaxf((float)widest4[2], (float)widest4[3])), lanes::Max());
       const float to_best = fmaxf(best, highest + (float)(widest > 0.0f ? __builtin_amdgcn_frexp_expf(widest) : -24));
       if (__builtin_amdgcn_ballot_w64(to_best > best)) {
         const float alpha = to_best > best ? __builtin_amdgcn_exp2f(best - to_best) : 1.0f;
@@ -286,19 +325,38 @@ __global__ __launch_bounds__(64 * kWaves) void paged_kernel(PagedArgs p) {
         }
       }
       const float base = best == -INFINITY ? 0.0f : best;
+      u32x2_t weights[SETS][G];  // times the scales, four in binary16
+#pragma unroll
+      for (int q = 0; q < SETS; ++q) {
+        half4_t ps[G];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float w = __builtin_amdgcn_exp2f(score[q][e] - base);
+          sum += w;
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            ps[g][e] = (half_t)(w * (float)vs[q][g][e]);
+            off[g] = __builtin_fmaf(w, (float)vz[q][g][e], off[g]);
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) weights[q][g] = __builtin_bit_cast(u32x2_t, ps[g]);
+      }
+      if (next >= 0) wait_for_requests<kKeyLoads>();
+      else wait_for_requests<0>();
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         half8_t pop[G];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int t = 2 * u + (e >> 2);
-          const float w = __builtin_amdgcn_exp2f(score[t][e & 3] - base);
-          sum += w;
+        for (int g = 0; g < G; ++g) {
+          u32x4_t x;
 #pragma unroll
-          for (int g = 0; g < G; ++g) {
-            pop[g][e] = (half_t)(w * (float)vs[g][t][e & 3]);
-            off[g] = __builtin_fmaf(w, (float)vz[g][t][e & 3], off[g]);
+          for (int h = 0; h < 2; ++h) {
+            const int t = 2 * u + h;
+            x[2 * h] = TP == 1 || mine == t % TP ? weights[t / TP][g][0] : 0u;
+            x[2 * h + 1] = TP == 1 || mine == t % TP ? weights[t / TP][g][1] : 0u;
           }
+          pop[g] = __builtin_bit_cast(half8_t, x);
         }
         // rows of the keys 4 kg + e of both sixteens, this lane's piece of each
         uint32_t row[8][(G + 1) / 2];
@@ -330,30 +388,82 @@ __global__ __launch_bounds__(64 * kWaves) void paged_kernel(PagedArgs p) {
           }
         }
       }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the values have been read
+      if (next >= 0) request_values(next);
+      here = next;
     }
-    sum = over_quarters_sum(sum);
+    // the columns of a head together, its sums over all quarters of the keys
+    const auto add_columns = [](float v) __attribute__((always_inline)) {
+      if constexpr (COLUMNS <= 4) v += lanes::from<0x124>(v);
+      if constexpr (COLUMNS <= 8) v += lanes::from<0x128>(v);
+      return v;
+    };
+    sum = over_head<COLUMNS>(sum, lanes::Add());
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      off[g] = over_quarters_sum(off[g]);
+      off[g] = over_head<COLUMNS>(off[g], lanes::Add());
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[g][j][e] = __builtin_fmaf(o[g][j][e], j % 2 ? 0x1p20f : 0x1p24f, off[g]);
+        for (int e = 0; e < 4; ++e) o[g][j][e] = __builtin_fmaf(add_columns(o[g][j][e]), j % 2 ? 0x1p20f : 0x1p24f, off[g]);
     }
-    // o[g][j][e]: value 64 g + 16 kg + 4 e + j of head m
-    if (from == 0 && to == n_pages) {
-      if (m < columns) {
-        const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-        T* const out = (T*)a.ctx + (int64_t)r * a.ldc + (int64_t)(head0 + m) * D + 16 * kg;
-        typedef T four_t __attribute__((ext_vector_type(4)));
+    // o[g][j][e]: value 64 g + 16 kg + 4 e + j of the lane's head
+    bool whole = from == 0 && to == n_pages, writes = m < columns;
+    if (wg_begin >= start && wg_end <= start + n_pages) {
+      // all four wavefronts have parts of this request and nothing else: together they are one
+      float* const meet = reinterpret_cast<float*>(lds);  // [4][columns][D], then [4][columns][2]
+      float* const meet_ml = meet + kWaves * COLUMNS * D;
+      static_assert(kWaves * COLUMNS * (D + 2) * 4 <= kWaves * kBytes, "the sums take the place of the pages");
+      __syncthreads();  // all pages have been read
+      if (writes) {
+        float* const out = meet + (wave * COLUMNS + m) * D + 16 * kg;
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<four_t*>(out + 64 * g + 4 * e) =
-                four_t{(T)(o[g][0][e] * inv), (T)(o[g][1][e] * inv), (T)(o[g][2][e] * inv), (T)(o[g][3][e] * inv)};
+          for (int e = 0; e < 4; ++e) *reinterpret_cast<f32x4_t*>(out + 64 * g + 4 * e) = f32x4_t{o[g][0][e], o[g][1][e], o[g][2][e], o[g][3][e]};
+        if (kg == 0) meet_ml[(wave * COLUMNS + m) * 2] = best, meet_ml[(wave * COLUMNS + m) * 2 + 1] = sum;
       }
-    } else if (m < columns) {
+      __syncthreads();
+      whole = wg_begin == start && wg_end == start + n_pages;
+      const int64_t slot = ((int64_t)stream * p.workers + worker - wave) * 2 + (start < wg_begin ? 0 : 1);
+      for (int x = threadIdx.x; x < columns * (D / 4); x += 64 * kWaves) {
+        const int c = x / (D / 4), d = x % (D / 4) * 4;
+        float top = -INFINITY, total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, meet_ml[(w * COLUMNS + c) * 2]);
+        const float base = top == -INFINITY ? 0.0f : top;
+        f32x4_t y = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          const float f = __builtin_amdgcn_exp2f(meet_ml[(w * COLUMNS + c) * 2] - base);
+          const f32x4_t v = *reinterpret_cast<const f32x4_t*>(meet + (w * COLUMNS + c) * D + d);
+          total = __builtin_fmaf(f, meet_ml[(w * COLUMNS + c) * 2 + 1], total);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(f, v[e], y[e]);
+        }
+        if (whole) {
+          const float inv = total != 0.0f ? 1.0f / total : 0.0f;
+          typedef T four_t __attribute__((ext_vector_type(4)));
+          *reinterpret_cast<four_t*>((T*)a.ctx + (int64_t)r * a.ldc + (int64_t)(head0 + c) * D + d) =
+              four_t{(T)(y[0] * inv), (T)(y[1] * inv), (T)(y[2] * inv), (T)(y[3] * inv)};
+        } else {
+          *reinterpret_cast<f32x4_t*>(p.sums + (slot * p.columns + c) * D + d) = y;
+          if (d == 0) p.ml[(slot * p.columns + c) * 2] = top, p.ml[(slot * p.columns + c) * 2 + 1] = total;
+        }
+      }
+      return;
+    }
+    if (whole && writes) {
+      const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+      T* const out = (T*)a.ctx + (int64_t)r * a.ldc + (int64_t)(head0 + m) * D + 16 * kg;
+      typedef T four_t __attribute__((ext_vector_type(4)));
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<four_t*>(out + 64 * g + 4 * e) =
+              four_t{(T)(o[g][0][e] * inv), (T)(o[g][1][e] * inv), (T)(o[g][2][e] * inv), (T)(o[g][3][e] * inv)};
+    } else if (writes) {
       // (a worker has two such requests at most: the one that its run begins in and the one that it ends in)
       const int64_t slot = ((int64_t)stream * p.workers + worker) * 2 + (start < begin ? 0 : 1);
       float* const out = p.sums + (slot * p.columns + m) * D + 16 * kg;
@@ -373,16 +483,20 @@ __global__ __launch_bounds__(64 * kWaves) void paged_kernel(PagedArgs p) {
 
 constexpr int kJoin = 512;
 
-// The parts of a request's sums, of one stream, whose workers lie side by side; requests without a position.
+// The parts of a request's sums, of one stream, whose workers lie side by side: 4 `quads` values a workgroup, every 512 / quads-th part a
+// thread; zeros for requests without a position.
 template <typename T>
-__global__ __launch_bounds__(kJoin) void paged_join_kernel(PagedArgs p) {
-  __shared__ int before_of[2];
-  __shared__ float part[kJoin * 4];
+__global__ __launch_bounds__(kJoin) void paged_join_kernel(PagedArgs p, int chunks, int quads) {
+  __shared__ int pages[2];
+  __shared__ float best_of[kJoin], sum_of[kJoin];
+  __shared__ f32x4_t o_of[kJoin];
   const awq_paged_attention_args& a = p.a;
-  const int r = blockIdx.x / p.streams, stream = blockIdx.x % p.streams, tid = threadIdx.x, D = a.dim;
+  const int chunk = blockIdx.x % chunks, stream = blockIdx.x / chunks % p.streams, r = blockIdx.x / chunks / p.streams;
+  const int tid = threadIdx.x, D = a.dim, shares = kJoin / quads;
   const int tiles = p.streams / a.kv_heads, group = a.heads / a.kv_heads;
   const int head0 = stream / tiles * group + stream % tiles * kColumns, columns = min(kColumns, group - stream % tiles * kColumns);
-  if (tid < 2) before_of[tid] = 0;
+  const int value = (chunk * quads + tid % quads) * 4, share = tid / quads;  // of all columns' values
+  if (tid < 2) pages[tid] = 0;
   __syncthreads();
   int before = 0, all = 0;
   for (int i = tid; i < a.n_requests; i += kJoin) {
@@ -390,68 +504,77 @@ __global__ __launch_bounds__(kJoin) void paged_join_kernel(PagedArgs p) {
     all += n;
     if (i < r) before += n;
   }
-  if (all) atomicAdd(&before_of[0], all);
-  if (before) atomicAdd(&before_of[1], before);
+  if (all) atomicAdd(&pages[0], all);
+  if (before) atomicAdd(&pages[1], before);
   const int n_pages = pages_of(a, r);
   __syncthreads();
-  all = before_of[0];
-  const int begin = before_of[1], end = begin + n_pages;
-  T* const out = (T*)a.ctx + (int64_t)r * a.ldc + (int64_t)head0 * D;
+  all = pages[0];
+  const int begin = pages[1], end = begin + n_pages, each = run_of(all, p.workers);
+  T* const out = (T*)a.ctx + (int64_t)r * a.ldc + (int64_t)head0 * D + value;
+  typedef T four_t __attribute__((ext_vector_type(4)));
   if (n_pages == 0) {
-    for (int i = tid; i < columns * D; i += kJoin) out[i] = (T)0.0f;
+    if (share == 0 && value < columns * D) *reinterpret_cast<four_t*>(out) = four_t{(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
     return;
   }
-  // the worker of a page: the last whose first page is not behind it
-  const auto worker_of = [&](int page) {
-    int w = (int)((int64_t)page * p.workers / all);
-    while (w + 1 < p.workers && first_page(w + 1, all, p.workers) <= page) ++w;
-    while (first_page(w, all, p.workers) > page) --w;
-    return w;
+  const int first = begin / each, last = (end - 1) / each;
+  // workgroups whose four workers have pages of this request alone have left one sum: workers from .. to
+  int from = (first + kWaves - 1) / kWaves * kWaves, to = (last + 1) / kWaves * kWaves;
+  if (from * each < begin) from += kWaves;
+  if (to > from && min(to * each, all) > end) to -= kWaves;
+  if (to < from) from = to = last + 1;
+  if (first == last || (from == first && to == last + 1 && to - from == kWaves)) return;  // one worker or workgroup had all of it
+  const int singles = from - first, wholes = (to - from) / kWaves, parts = singles + wholes + (last + 1 - to);
+  const auto slot_of = [&](int i) {
+    const int w = i < singles ? first + i : i < singles + wholes ? from + (i - singles) * kWaves : to + i - singles - wholes;
+    return ((int64_t)stream * p.workers + w) * 2 + (w == first);  // (it begins in the first and ran on in the others)
   };
-  const int first = worker_of(begin), last = worker_of(end - 1);
-  if (first == last) return;  // one worker had all of it
-  const int64_t at = (int64_t)stream * p.workers;
-  const auto slot_of = [&](int w) { return (at + w) * 2 + (w == first); };  // (it begins in the first and ran on in the others)
-  const int quads = columns * D / 4, shares = max(1, kJoin / quads);
-  for (int q0 = 0; q0 < quads; q0 += kJoin) {
-    const int share = quads >= kJoin ? 0 : tid / quads, quad = quads >= kJoin ? q0 + tid : tid % quads;
-    const bool mine = quad < quads && share < shares;
-    const int head = min(quad * 4 / D, columns - 1);
-    float best = -INFINITY, sum = 0.0f;
-    f32x4_t o = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    if (mine) {
-      for (int w = first; w <= last; ++w) {
-        if (first_page(w, all, p.workers) == first_page(w + 1, all, p.workers)) continue;
-        best = fmaxf(best, p.ml[(slot_of(w) * p.columns + head) * 2]);
-      }
-      const float base = best == -INFINITY ? 0.0f : best;
-      for (int w = first + share; w <= last; w += shares) {
-        if (first_page(w, all, p.workers) == first_page(w + 1, all, p.workers)) continue;
-        const int64_t s = slot_of(w) * p.columns + head;
-        const float f = __builtin_amdgcn_exp2f(p.ml[s * 2] - base);
-        sum = __builtin_fmaf(f, p.ml[s * 2 + 1], sum);
-        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(p.sums + s * D + quad * 4 % D);
+  const int head = min(value / D, columns - 1);
+  f32x4_t o = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  float best = -INFINITY, sum = 0.0f;
+  const auto add = [&](float m, float l, f32x4_t v) __attribute__((always_inline)) {
+    const float to = fmaxf(best, m), base = to == -INFINITY ? 0.0f : to;
+    const float f = __builtin_amdgcn_exp2f(best - base), g = __builtin_amdgcn_exp2f(m - base);
+    best = to;
+    sum = __builtin_fmaf(g, l, sum * f);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(f, v[e], o[e]);
-      }
-    }
-    if (shares > 1) {
-      __shared__ float sum_of[kJoin];
-      *reinterpret_cast<f32x4_t*>(part + tid * 4) = o;
-      sum_of[tid] = sum;
-      __syncthreads();
-      if (mine && share == 0)
-        for (int s = 1; s < shares; ++s) {
-          o = o + *reinterpret_cast<const f32x4_t*>(part + (s * quads + quad) * 4);
-          sum += sum_of[s * quads + quad];
-        }
-    }
-    if (mine && share == 0) {
-      const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) out[quad * 4 + e] = (T)(o[e] * inv);
-    }
+    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(g, v[e], o[e] * f);
+  };
+#pragma unroll 4
+  for (int i = share; i < parts; i += shares) {
+    const int64_t s = slot_of(i) * p.columns + head;
+    add(p.ml[s * 2], p.ml[s * 2 + 1], *reinterpret_cast<const f32x4_t*>(p.sums + s * D + value % D));
   }
+  best_of[tid] = best;
+  sum_of[tid] = sum;
+  o_of[tid] = o;
+  __syncthreads();
+  if (share || value >= columns * D) return;
+  for (int i = 1; i < min(shares, parts); ++i) add(best_of[i * quads + tid], sum_of[i * quads + tid], o_of[i * quads + tid]);
+  const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+  *reinterpret_cast<four_t*>(out) = four_t{(T)(o[0] * inv), (T)(o[1] * inv), (T)(o[2] * inv), (T)(o[3] * inv)};
+}
+
+template <typename T, int D>
+void launch_pages(const PagedArgs& p, dim3 grid, hipStream_t st) {
+  if (p.columns <= 4) hipLaunchKernelGGL((paged_kernel<T, D, 4>), grid, dim3(64 * kWaves), 0, st, p);
+  else if (p.columns <= 8) hipLaunchKernelGGL((paged_kernel<T, D, 8>), grid, dim3(64 * kWaves), 0, st, p);
+  else hipLaunchKernelGGL((paged_kernel<T, D, 16>), grid, dim3(64 * kWaves), 0, st, p);
+}
+
+template <typename T>
+int launch(const PagedArgs& p, hipStream_t st) {
+  const dim3 grid((unsigned)(p.workers / kWaves * p.streams));
+  if (p.a.dim == 64) launch_pages<T, 64>(p, grid, st);
+  else if (p.a.dim == 128) launch_pages<T, 128>(p, grid, st);
+  else launch_pages<T, 256>(p, grid, st);
+  AWQ_HIP_TRY(hipGetLastError());
+  // wide pieces of a request's values where the workers are cut over many requests, few parts each; narrow ones, whose threads share the parts,
+  // where they are cut over few
+  const int quads = p.workers / kWaves > 16 * p.a.n_requests ? 32 : 128;
+  const int chunks = (p.columns * p.a.dim + 4 * quads - 1) / (4 * quads);
+  hipLaunchKernelGGL(paged_join_kernel<T>, dim3((unsigned)(p.a.n_requests * p.streams * chunks)), dim3(kJoin), 0, st, p, chunks, quads);
+  AWQ_HIP_TRY(hipGetLastError());
+  return AWQ_OK;
 }
 
 }  // namespace
@@ -462,7 +585,6 @@ int64_t paged_workspace_bytes(int n_requests, int heads, int kv_heads, int dim, 
 }
 
 int launch_paged_attention(const awq_paged_attention_args& u, bool bf16, hipStream_t st) {
-  if (u.n_requests == 0) return AWQ_OK;
   PagedArgs p;
   p.a = u;
   p.streams = streams_of(u.heads, u.kv_heads);
@@ -470,14 +592,6 @@ int launch_paged_attention(const awq_paged_attention_args& u, bool bf16, hipStre
   p.columns = columns_of(u.heads / u.kv_heads);
   p.sums = (float*)u.workspace;
   p.ml = p.sums + (int64_t)p.streams * p.workers * 2 * p.columns * u.dim;
-  const dim3 grid((unsigned)(p.workers / kWaves * p.streams)), block(64 * kWaves);
-  const auto kernel = bf16 ? (u.dim == 64 ? paged_kernel<bf16_t, 64> : u.dim == 128 ? paged_kernel<bf16_t, 128> : paged_kernel<bf16_t, 256>)
-                           : (u.dim == 64 ? paged_kernel<half_t, 64> : u.dim == 128 ? paged_kernel<half_t, 128> : paged_kernel<half_t, 256>);
-  hipLaunchKernelGGL(kernel, grid, block, 0, st, p);
-  AWQ_HIP_TRY(hipGetLastError());
-  AWQ_REQUIRE((int64_t)u.n_requests * p.streams < (1ll << 31), "too many requests and heads");
-  const dim3 join((unsigned)(u.n_requests * p.streams));
-  hipLaunchKernelGGL(bf16 ? paged_join_kernel<bf16_t> : paged_join_kernel<half_t>, join, dim3(kJoin), 0, st, p);
-  AWQ_HIP_TRY(hipGetLastError());
-  return AWQ_OK;
+  AWQ_REQUIRE((int64_t)u.n_requests * p.streams * p.columns * u.dim / 64 < (1ll << 31), "too many requests and heads");
+  return bf16 ? launch<bf16_t>(p, st) : launch<half_t>(p, st);
 }
