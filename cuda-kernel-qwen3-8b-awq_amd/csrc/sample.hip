@@ -5,15 +5,19 @@
 namespace {
 
 // Weights go into bins of a quarter of a nat, y = 4 l / T, bin floor(y); of a row or a part of it only the 256 bins from its largest logit's down
-// are looked at: what lies further is below e^-63, and 64 bits of a sum would not show it.  Within a bin a weight is e^((y - bin - 1) / 4), between e^(-1/4) and 1, as a whole multiple of 2^-36, so that
-// sums do not depend on their order; bins are joined in 64-bit floating point.  (Tokens with the largest logit are all in the first bin: their sums
-// are exact, and uniform numbers such as 1/2 fall between two of them as they should.)
+// are looked at: what lies further is below e^-63, and 64 bits of a sum would not show it.  Within a bin a weight is e^((y - bin - 1) / 4),
+// between e^(-1/4) and 1, as a whole multiple of 2^-36, so that sums do not depend on their order; bins are joined in 64-bit floating point.
+// (Tokens with the largest logit are all in the first bin: their sums are exact, and uniform numbers such as 1/2 fall between two of them as
+// they should.)
 //   scan_kernel    parts of 8,192 logits: largest, sum of weights, and where a row is filtered a histogram, sums and counts by bin
 //   choose_kernel  a workgroup a row: the bin in which the tokens kept end, the order within that bin alone, the part that the uniform
 //                  number falls in, and the token in that part.
-constexpr int kPart = 8192, kScan = 256, kChoose = 1024, kBins = 256, kChunk = 32, kHeld = 8192, kRanked = 512;
+constexpr int kPart = 8192, kScan = 256, kChoose = 512, kBins = 256, kChunk = 32, kHeld = 8192, kFew = 512, kMostParts = 64;
+constexpr int kMostChunks = kMostParts * kPart / kChunk, kCopies = 8;
 constexpr int kFixed = 36, kCountShift = 50;
-constexpr double kFarthest = 0x1p50;  // of y: logits beyond 2^48 T count as that
+constexpr uint64_t kSumMask = (1ull << kCountShift) - 1;
+constexpr double kUnit = 1.0 / (double)(1ll << kFixed);
+constexpr double kRound = 0x1.8p16;  // numbers of its size are 2^-36 apart
 
 struct Part {
   float largest;
@@ -24,12 +28,20 @@ struct SampleArgs {
   awq_sample_args a;
   int parts, chunks;
   Part* part;           // [rows][parts]
-  uint64_t* histogram;  // [rows][parts][kBins]: count << 50 | sum, at bin mod 256
+  uint64_t* histogram;  // [rows][parts][kBins]: count << 50 | sum, from the bin of the part's largest down
   float* chunk;         // [rows][chunks]: largest of 32 logits
 };
 
+// a value that all lanes have, in scalar registers: branches on it are the wavefront's, and it takes no lane's register through them
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(uniform(__float_as_uint(v))); }
+__device__ __forceinline__ uint64_t uniform(uint64_t v) { return (uint64_t)uniform((uint32_t)(v >> 32)) << 32 | uniform((uint32_t)v); }
+__device__ __forceinline__ double uniform(double v) { return __longlong_as_double((long long)uniform((uint64_t)__double_as_longlong(v))); }
+
 struct Row {
   double per_t;  // 4 / T
+  float limit;   // logits beyond 2^48 T count as that
   float top_p, min_p;
   int top_k;  // 0: not limited
   bool greedy, filtered;
@@ -38,7 +50,8 @@ __device__ __forceinline__ Row row_of(const awq_sample_args& a, int64_t row) {
   Row r;
   const float t = a.temperature ? a.temperature[row] : 1.0f;
   r.greedy = !(t > 0.0f);
-  r.per_t = 4.0 / (double)t;
+  r.per_t = uniform(4.0 / (double)t);
+  r.limit = fminf(0x1p48f * t, 3.4028234663852886e38f);
   r.top_k = a.top_k ? a.top_k[row] : 0;
   if (r.top_k < 0 || r.top_k >= a.vocab) r.top_k = 0;
   r.top_p = a.top_p ? a.top_p[row] : 1.0f;
@@ -50,33 +63,39 @@ __device__ __forceinline__ Row row_of(const awq_sample_args& a, int64_t row) {
   return r;
 }
 
+__device__ __forceinline__ double y_of(float l, const Row& r) { return (double)fminf(fmaxf(l, -r.limit), r.limit) * r.per_t; }
+__device__ __forceinline__ double bin_of(float l, const Row& r) { return floor(y_of(l, r)); }
 struct Binned {
-  double bin, weight;  // weight relative to e^((bin + 1) / 4), a whole multiple of 2^-36
+  double bin, rounded;  // rounded: kRound + the weight relative to e^((bin + 1) / 4)
 };
-constexpr double kRound = 0x1.8p16;  // numbers of its size are 2^-36 apart
-__device__ __forceinline__ double bin_of(double l, double per_t) { return floor(fmin(fmax(l * per_t, -kFarthest), kFarthest)); }
-__device__ __forceinline__ Binned binned(float l, double per_t) {
-  const double y = fmin(fmax((double)l * per_t, -kFarthest), kFarthest), b = floor(y);
-  // e^(f - 1/8), f within 1/8 of 0: the series up to f^9 / 9!, the next term is below 3e-16
-  const double f = (y - b) * 0.25 - 0.125;
-  double e = 1.0 / 362880.0;
-  e = fma(e, f, 1.0 / 40320.0);
-  e = fma(e, f, 1.0 / 5040.0);
-  e = fma(e, f, 1.0 / 720.0);
-  e = fma(e, f, 1.0 / 120.0);
-  e = fma(e, f, 1.0 / 24.0);
-  e = fma(e, f, 1.0 / 6.0);
-  e = fma(e, f, 0.5);
-  e = fma(e, f, 1.0);
-  e = fma(e, f, 1.0);
-  return {b, fma(e, 0.88249690258459540286, kRound) - kRound};  // e^(-1/8)
+__device__ __forceinline__ Binned binned(float l, const Row& r) {
+  const double y = y_of(l, r), b = floor(y), x = y - b;
+  // e^((x - 1) / 4) for x from 0 to 1: the polynomial through its values at the seven Chebyshev points, within 1.7e-12
+  double e = 2.9938727103789073e-07;
+  e = fma(e, x, 6.288293243577365e-06);
+  e = fma(e, x, 0.00012679210980033013);
+  e = fma(e, x, 0.002028115011608631);
+  e = fma(e, x, 0.02433752648211561);
+  e = fma(e, x, 0.1947001956419453);
+  e = fma(e, x, 0.7788007830726902);
+  return {b, e + kRound};
 }
-__device__ __forceinline__ uint64_t fixed_of(double weight) { return (uint64_t)__double_as_longlong(weight + kRound) & ((1ull << 51) - 1); }
-__device__ __forceinline__ int place_of(double bin) { return (int)((int64_t)bin & (kBins - 1)); }
+// the weight as a multiple of 2^-36, and as a number
+__device__ __forceinline__ uint64_t fixed_of(const Binned& b) { return (uint64_t)__double_as_longlong(b.rounded) & ((1ull << 51) - 1); }
+__device__ __forceinline__ double weight_of(const Binned& b) { return b.rounded - kRound; }
 
 __device__ __forceinline__ float logit(float v) { return v != v ? -INFINITY : v + 0.0f; }  // (-0 as 0)
 // of a row with logits of +infinity those share the weight
 __device__ __forceinline__ float finite(float v, bool infinite) { return infinite ? (v == INFINITY ? 0.0f : -INFINITY) : v; }
+
+// order of logits as whole numbers
+__device__ __forceinline__ uint32_t key_of(float l) {
+  const uint32_t u = __float_as_uint(l);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+// order of the tokens: falling logits, rising ids; larger numbers first
+__device__ __forceinline__ uint64_t order_of(float l, uint32_t id) { return (uint64_t)key_of(l) << 32 | (uint32_t)~id; }
 
 template <typename T, int N>
 struct Some {
@@ -91,16 +110,14 @@ __global__ __launch_bounds__(kScan) void scan_kernel(SampleArgs s) {
   __shared__ float largest_of[kScan / 64];
   __shared__ int first_of[kScan / 64];
   __shared__ double sum_of[kScan / 64];
-  __shared__ unsigned long long bins[kScan / 64][kBins];
+  __shared__ unsigned long long bins[kBins * kCopies];  // (copies by lane: lanes that meet in a bin wait for each other)
   __shared__ double table[kBins];
   const awq_sample_args& a = s.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x / s.parts;
   const int part = blockIdx.x % s.parts;
-  const Row r = row_of(a, row);
   const T* const x = (const T*)a.logits + row * a.ld;
   float v[L][W];
-  float largest = -INFINITY;
 #pragma unroll
   for (int i = 0; i < L; ++i) {
     const int64_t at = (int64_t)part * kPart + (i * kScan + tid) * W;
@@ -113,6 +130,15 @@ __global__ __launch_bounds__(kScan) void scan_kernel(SampleArgs s) {
       for (int e = 0; e < W; ++e) v[i][e] = at + e < a.vocab ? logit((float)x[at + e]) : -INFINITY;
     }
   }
+  const Row r = row_of(a, row);
+  if (!r.greedy) {
+    if (r.filtered) {
+      for (int b = tid; b < kBins * kCopies; b += kScan) bins[b] = 0;
+    } else {
+      table[tid] = exp(-0.25 * tid);
+    }
+  }
+  float largest = -INFINITY;
 #pragma unroll
   for (int i = 0; i < L; ++i) {
     float m = v[i][0];
@@ -125,9 +151,6 @@ __global__ __launch_bounds__(kScan) void scan_kernel(SampleArgs s) {
       if (tid % LANES == 0 && at < s.chunks) s.chunk[row * s.chunks + at] = m;
     }
   }
-  if (r.filtered && !r.greedy)
-    for (int b = lane; b < kBins; b += 64) bins[wave][b] = 0;
-  table[tid] = exp(-0.25 * tid);
   largest = lanes::maximum<64>(largest);
   if (lane == 0) largest_of[wave] = largest;
   __syncthreads();
@@ -148,22 +171,25 @@ __global__ __launch_bounds__(kScan) void scan_kernel(SampleArgs s) {
     out.first = min(min(first_of[0], first_of[1]), min(first_of[2], first_of[3]));
   } else if (largest > -INFINITY) {
     const bool infinite = largest == INFINITY;
-    const double top = bin_of(infinite ? 0.0 : (double)largest, r.per_t);
+    const double top = bin_of(finite(largest, infinite), r);
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < L; ++i)
 #pragma unroll
       for (int e = 0; e < W; ++e) {
-        const Binned b = binned(finite(v[i][e], infinite), r.per_t);
+        const float l = finite(v[i][e], infinite);
+        const Binned b = binned(l, r);
         const double below = top - b.bin;
-        if (below >= kBins || finite(v[i][e], infinite) == -INFINITY) continue;
-        if (r.filtered) atomicAdd(&bins[wave][place_of(b.bin)], (1ull << kCountShift) | fixed_of(b.weight));
-        else sum += b.weight * table[(int)below];
+        if (!(below < kBins) || l == -INFINITY) continue;
+        if (r.filtered) atomicAdd(&bins[(int)below * kCopies + lane % kCopies], (1ull << kCountShift) | fixed_of(b));
+        else sum += weight_of(b) * table[(int)below];
       }
     if (r.filtered) {
       __syncthreads();
-      uint64_t* const to = s.histogram + ((int64_t)row * s.parts + part) * kBins;
-      to[tid] = (bins[0][tid] + bins[1][tid]) + (bins[2][tid] + bins[3][tid]);
+      unsigned long long all = 0;
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c) all += bins[tid * kCopies + (c + tid) % kCopies];
+      s.histogram[(row * s.parts + part) * kBins + tid] = all;
     } else {
 #pragma unroll
       for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
@@ -175,12 +201,68 @@ __global__ __launch_bounds__(kScan) void scan_kernel(SampleArgs s) {
   if (tid == 0) s.part[row * s.parts + part] = out;
 }
 
-constexpr int kMostParts = 64;
+struct ChooseMemory {
+  uint64_t held[kHeld];       // order of the tokens of a bin, where they are so few
+  uint16_t list[kMostChunks]; // chunks that have some
+  uint64_t few[kFew], few_weight[kFew];
+  uint64_t digit[kBins];
+  uint32_t digit_count[kBins];
+  uint64_t word[2], in_bin[kMostParts];
+  uint64_t fixed[kBins];
+  uint32_t bin_count[kBins];
+  double table[kBins], part_sum[kMostParts], wave_sum[kChoose / 64];
+  Part part[kMostParts];
+  int behind[kMostParts];
+  uint32_t held_count, list_count, few_count;
+  int pick, last;
+};
 
-// order of the tokens: falling logits, rising ids; larger numbers first
-__device__ __forceinline__ uint64_t order_of(float l, uint32_t id) {
-  const uint32_t u = __float_as_uint(l);
-  return (uint64_t)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (uint32_t)~id;
+template <typename T>
+__device__ __forceinline__ T sums_of_wave(T v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const T u = __shfl_up(v, off, 64);
+    if (lane >= off) v += u;
+  }
+  return v;
+}
+
+// The first of 256 entries, four a lane, at which `full` holds of the sums up to it (itself included), and the sums ahead of it; 256: none.
+// Every wavefront finds it for itself.
+template <typename S>
+struct Found {
+  int at;
+  S sum;
+  uint32_t count;
+};
+template <typename S, typename F>
+__device__ __forceinline__ Found<S> first_full(const S (&sum)[4], const uint32_t (&count)[4], F full) {
+  const int lane = threadIdx.x & 63;
+  const S mine = ((sum[0] + sum[1]) + sum[2]) + sum[3];
+  const uint32_t many = count[0] + count[1] + count[2] + count[3];
+  S s = sums_of_wave(mine) - mine;
+  if constexpr (__is_same(S, double)) {  // (the sums ahead as they are formed, not as a difference)
+    const S up = __shfl_up(sums_of_wave(mine), 1, 64);
+    s = lane ? up : 0.0;
+  }
+  uint32_t n = sums_of_wave(many) - many;
+  int at = 4;
+  S before = s;
+  uint32_t before_count = n;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s += sum[i];
+    n += count[i];
+    if (at == 4) {
+      if (full(s, n)) at = i;
+      else before = s, before_count = n;
+    }
+  }
+  const unsigned long long any = __builtin_amdgcn_ballot_w64(at < 4);
+  if (any == 0) return {kBins, (S)0, 0};
+  const int from = __builtin_ctzll(any);
+  return {uniform(4 * from + __shfl(at, from, 64)), uniform(__shfl(before, from, 64)), uniform((uint32_t)__shfl((int)before_count, from, 64))};
 }
 
 template <typename T>
@@ -189,135 +271,194 @@ struct Choose {
   const Row& r;
   const T* x;
   const float* chunk;
-  double top;      // the bin of the row's largest
+  ChooseMemory& m;
+  float largest;  // of the row
+  double top;     // its bin
   bool infinite;
-  // shared memory
-  uint64_t* held;        // [kHeld] order of the tokens of a bin
-  uint64_t* digit;       // [256] sums
-  uint32_t* digit_count; // [256]
-  uint64_t* words;       // [4]
-  uint32_t* count;
 
   __device__ __forceinline__ float at(int i) const { return finite(logit((float)x[i]), infinite); }
   // distance of a logit's bin from the row's first; 256: further or no weight
   __device__ __forceinline__ int below(const Binned& b, float l) const {
     const double d = top - b.bin;
-    return l == -INFINITY || d >= kBins ? kBins : (int)d;
+    return l == -INFINITY || !(d < kBins) ? kBins : (int)d;
   }
-  // every token of bin j: f(order, fixed weight); out of the row, by runs of 32 that can have one
+  // the lowest order of a logit in bin j or ahead of it, by 64 guesses at a time
+  __device__ __forceinline__ uint32_t lowest_key(int j) const {
+    uint32_t lo = key_of(-INFINITY), hi = uniform(key_of(largest));  // not in it, in it
+    for (int turn = 0; turn < 6 && hi - lo > 1; ++turn) {  // (2^32 in six turns)
+      const uint32_t step = (hi - lo + 63) / 64, guess = lo + step * ((threadIdx.x & 63) + 1);
+      const bool in = guess >= hi || top - bin_of(logit_of(guess), r) <= j;
+      const uint32_t first = __builtin_ctzll(__builtin_amdgcn_ballot_w64(in) | 1ull << 63);  // (the last lane's guess is not below hi)
+      hi = min(hi, lo + step * (first + 1));
+      lo = lo + step * first;
+    }
+    return hi;
+  }
+  // every token of the orders a .. b - 1: f(order); out of the row, by the chunks listed, 16 bytes of a chunk a thread and four of them at once
   template <typename F>
-  __device__ __forceinline__ void each_of_row(int j, F f) const {
-    const int vocab = (int)s.a.vocab;
-    for (int c = threadIdx.x / kChunk; c < s.chunks; c += kChoose / kChunk) {
-      const float m = finite(chunk[c], infinite);
-      if (m == -INFINITY || top - bin_of((double)m, r.per_t) > j) continue;
-      const int i = c * kChunk + threadIdx.x % kChunk;
-      if (i >= vocab) continue;
-      const float l = at(i);
-      const Binned b = binned(l, r.per_t);
-      if (below(b, l) == j) f(order_of(l, i), fixed_of(b.weight));
+  __device__ __forceinline__ void each_of_row(uint64_t a, uint64_t b, F f) const {
+    constexpr int W = 16 / sizeof(T), LANES = kChunk / W, AT_ONCE = kChoose / LANES, U = 4;
+    typedef typename Some<T, W>::type vec_t;
+    const int vocab = (int)s.a.vocab, n = uniform((int)m.list_count), first = threadIdx.x / LANES, in_chunk = threadIdx.x % LANES * W;
+    for (int c0 = first; c0 < n; c0 += U * AT_ONCE) {
+      vec_t v[U];
+      int id[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        id[u] = c0 + u * AT_ONCE < n ? m.list[c0 + u * AT_ONCE] * kChunk + in_chunk : vocab;
+        if (id[u] + W <= vocab) v[u] = *reinterpret_cast<const vec_t*>(x + id[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (id[u] >= vocab) continue;
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          if (id[u] + W > vocab && id[u] + e >= vocab) continue;
+          const float l = finite(logit(id[u] + W <= vocab ? (float)v[u][e] : (float)x[id[u] + e]), infinite);
+          const uint64_t order = order_of(l, id[u] + e);
+          if (order >= a && order < b) f(order);
+        }
+      }
     }
   }
-  __device__ __forceinline__ float logit_of(uint64_t order) const {
-    const uint32_t u = order >> 32;
-    return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
-  }
+  __device__ __forceinline__ uint64_t fixed_at(uint64_t order) const { return fixed_of(binned(logit_of((uint32_t)(order >> 32)), r)); }
+  // every token of the orders a .. b - 1 of a bin of n; where they are not held a logit a thread (rows of some thousand equals)
   template <typename F>
-  __device__ __forceinline__ void each(int j, int n, F f) const {
-    if (n <= kHeld) {
-      for (int i = threadIdx.x; i < n; i += kChoose) f(held[i], fixed_of(binned(logit_of(held[i]), r.per_t).weight));
-    } else {
-      each_of_row(j, f);
+  __device__ __forceinline__ void each(int n, uint64_t a, uint64_t b, F f) const {
+    const int all = n <= kHeld ? n : uniform((int)m.list_count) * kChunk;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < all; i += kChoose) {
+      uint64_t order = 0;
+      if (n <= kHeld) {
+        order = m.held[i];
+      } else {
+        const int id = m.list[i / kChunk] * kChunk + i % kChunk;
+        if (id < (int)s.a.vocab) order = order_of(at(id), id);
+      }
+      if (order >= a && order < b) f(order);
     }
   }
-  __device__ __forceinline__ void gather(int j, int n) const {
+  // the chunks of bin j's n tokens, and the tokens themselves where they are few; a, b: their orders
+  __device__ __forceinline__ void gather(int j, int n, uint64_t& a, uint64_t& b) const {
+    const uint32_t low = lowest_key(j);
+    a = (uint64_t)low << 32;
+    b = (uint64_t)(j ? lowest_key(j - 1) : key_of(largest) + 1) << 32;
+    __syncthreads();  // the last bin's readers are done
+    if (threadIdx.x == 0) m.held_count = m.list_count = 0;
+    __syncthreads();
+    const int lane = threadIdx.x & 63;
+    for (int c0 = 0; c0 < s.chunks; c0 += kChoose) {
+      const int c = c0 + threadIdx.x;
+      const bool some = c < s.chunks && key_of(finite(chunk[min(c, s.chunks - 1)], infinite)) >= low;
+      const unsigned long long any = __builtin_amdgcn_ballot_w64(some);
+      if (any == 0) continue;
+      uint32_t to = 0;
+      if (lane == 0) to = atomicAdd(&m.list_count, (uint32_t)__builtin_popcountll(any));
+      to = __builtin_amdgcn_readfirstlane(to) + __builtin_popcountll(any & ((1ull << lane) - 1));
+      if (some) m.list[to] = (uint16_t)c;
+    }
+    __syncthreads();
     if (n > kHeld) return;
-    __syncthreads();
-    if (threadIdx.x == 0) *count = 0;
-    __syncthreads();
-    each_of_row(j, [&](uint64_t order, uint64_t) {
-      const uint32_t to = atomicAdd(count, 1u);
-      if (to < (uint32_t)kHeld) held[to] = order;
+    each_of_row(a, b, [&](uint64_t order) {
+      const uint32_t to = atomicAdd(&m.held_count, 1u);
+      if (to < (uint32_t)kHeld) m.held[to] = order;
     });
     __syncthreads();
   }
-  // Of the n tokens of bin j the one with which the count (sum == false: `need` of them) or the sum of the fixed weights (the first at
-  // which it reaches `reach`) is full.  words[0]: its order, 0 if there is none; words[1]: the sum up to it, itself included.
-  __device__ __forceinline__ void last_kept(int j, int n, bool by_sum, uint32_t need, double reach) const {
+  // Of a bin's n tokens, of the orders a .. b - 1, the one with which the count (by_sum == false: `need` of them) or the sum of the weights (the first at
+  // which it reaches `reach`) is full.  word[0]: its order, 0 if there is none; word[1]: the sum up to it, itself included.
+  // By digits of the order until few are left, then each of those against all others.
+  __device__ __forceinline__ void last_kept(int n, uint64_t a, uint64_t b, bool by_sum, uint32_t need, double reach) const {
+    const int tid = threadIdx.x, lane = tid & 63, all = n;
+    uint64_t ahead = 0;
+    uint32_t ahead_count = 0;
     __syncthreads();
-    if (threadIdx.x == 0) words[0] = words[1] = 0;
-    __syncthreads();
-    if (n <= kRanked) {
-      if ((int)threadIdx.x < n) {
-        const uint64_t mine = held[threadIdx.x], own = fixed_of(binned(logit_of(mine), r.per_t).weight);
-        uint32_t ahead = 0;
-        uint64_t sum = 0;
-        for (int i = 0; i < n; ++i)
-          if (held[i] > mine) ++ahead, sum += fixed_of(binned(logit_of(held[i]), r.per_t).weight);
-        const bool last = by_sum ? (double)sum < reach && (double)(sum + own) >= reach : ahead + 1 == need;
-        if (last) words[0] = mine, words[1] = sum + own;
-      }
+    if (tid == 0) m.word[0] = m.word[1] = 0;
+    while (n > kFew) {
+      const int shift = max(0, 56 - __builtin_clzll(b - a - 1));  // (b - a - 1) >> shift is below 256
       __syncthreads();
-      return;
-    }
-    uint64_t prefix = 0, sum = 0;
-    uint32_t before = 0;
-    for (int shift = 56; shift >= 0; shift -= 8) {
+      if (tid < kBins) m.digit[tid] = 0, m.digit_count[tid] = 0;
       __syncthreads();
-      if (threadIdx.x < 256) digit[threadIdx.x] = 0, digit_count[threadIdx.x] = 0;
-      __syncthreads();
-      each(j, n, [&](uint64_t order, uint64_t weight) {
-        if (shift < 56 && order >> (shift + 8) != prefix) return;
-        const int d = (int)(order >> shift) & 255;
-        atomicAdd((unsigned long long*)&digit[d], (unsigned long long)weight);
-        atomicAdd(&digit_count[d], 1u);
+      each(all, a, b, [&](uint64_t order) {
+        const int d = (int)((order - a) >> shift);
+        atomicAdd((unsigned long long*)&m.digit[d], (unsigned long long)fixed_at(order));
+        atomicAdd(&m.digit_count[d], 1u);
       });
       __syncthreads();
-      int d = 255;
-      for (; d > 0; --d) {  // (the same in every thread)
-        const bool full = by_sum ? (double)(sum + digit[d]) >= reach : before + digit_count[d] >= need;
-        if (full && digit_count[d]) break;
-        sum += digit[d];
-        before += digit_count[d];
-      }
-      prefix = prefix << 8 | (uint64_t)d;
+      uint64_t sum[4];
+      uint32_t count[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] = m.digit[255 - 4 * lane - i], count[i] = m.digit_count[255 - 4 * lane - i];
+      const Found<uint64_t> f = first_full(sum, count, [&](uint64_t su, uint32_t co) {
+        return by_sum ? (double)(ahead + su) >= reach : ahead_count + co >= need;
+      });
+      if (f.at == kBins) return;  // (a rounding away from all of them)
+      const uint64_t d = 255 - f.at;
+      ahead += f.sum;
+      ahead_count += f.count;
+      n = uniform((int)m.digit_count[d]);
+      a += d << shift;
+      if (b - a > 1ull << shift) b = a + (1ull << shift);
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-      const uint64_t own = fixed_of(binned(logit_of(prefix), r.per_t).weight);
-      words[0] = prefix;
-      words[1] = sum + own;
+    if (tid == 0) m.few_count = 0;
+    __syncthreads();
+    each(all, a, b, [&](uint64_t order) {
+      const uint32_t to = atomicAdd(&m.few_count, 1u);
+      if (to < (uint32_t)kFew) {
+        m.few[to] = order;
+        m.few_weight[to] = fixed_at(order);
+      }
+    });
+    __syncthreads();
+    n = uniform(min((int)m.few_count, kFew));
+    const int wide = n <= 8 ? 64 : kChoose >> (32 - __builtin_clz(n - 1));  // threads a token: 1 .. 64
+    static_assert(kFew <= kChoose && 8 * 64 <= kChoose, "a thread a token at least");
+    const int mine = tid / wide;
+    const uint64_t order = mine < n ? m.few[mine] : ~0ull;
+    uint64_t sum = 0;
+    uint32_t count = 0;
+    for (int i = tid % wide; i < n; i += wide)
+      if (m.few[i] > order) ++count, sum += m.few_weight[i];
+    for (int off = wide / 2; off > 0; off >>= 1) {
+      sum += __shfl_xor(sum, off, 64);
+      count += __shfl_xor(count, off, 64);
+    }
+    if (mine < n && tid % wide == 0) {
+      const uint64_t with = ahead + sum + m.few_weight[mine];
+      if (by_sum ? (double)(ahead + sum) < reach && (double)with >= reach : ahead_count + count + 1 == need) m.word[0] = order, m.word[1] = with;
     }
     __syncthreads();
   }
 };
 
+// (512 threads: at 1,024 a thread has 128 registers, fewer than it needs)
 template <typename T>
 __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
-  __shared__ uint64_t held[kHeld], digit[256], words[4], in_bin[kMostParts];
-  __shared__ uint32_t digit_count[256], count;
-  __shared__ double table[kBins], sums[kBins], part_sum[kMostParts], wave_sum[kChoose / 64];
-  __shared__ uint32_t counts[kBins];
-  __shared__ uint64_t fixed[kBins];
-  __shared__ Part parts[kMostParts];
-  __shared__ int pick, last;
+  __shared__ ChooseMemory m;
   const awq_sample_args& a = s.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = s.parts;
   const int64_t row = blockIdx.x;
+  if (tid < S) m.part[tid] = s.part[row * S + tid];
   const Row r = row_of(a, row);
-  if (tid < S) parts[tid] = s.part[row * S + tid];
-  if (tid < kBins) table[tid] = exp(-0.25 * tid);
-  if (tid == 0) pick = INT32_MAX, last = 0;
+  if (!r.greedy && tid < kBins) {
+    m.table[tid] = exp(-0.25 * tid);
+    m.fixed[tid] = 0;
+    m.bin_count[tid] = 0;
+  }
+  if (tid < kMostParts) m.in_bin[tid] = 0;
+  if (tid == 0) m.pick = INT32_MAX, m.last = 0;
   __syncthreads();
   float largest = -INFINITY;
-  for (int i = 0; i < S; ++i) largest = fmaxf(largest, parts[i].largest);
+  for (int i = 0; i < S; ++i) largest = fmaxf(largest, m.part[i].largest);
+  largest = uniform(largest);
   if (r.greedy || largest == -INFINITY) {
     if (tid == 0) {
       int id = 0;
       if (largest > -INFINITY)
         for (int i = 0; i < S; ++i)
-          if (parts[i].largest == largest) {
-            id = parts[i].first;
+          if (m.part[i].largest == largest) {
+            id = m.part[i].first;
             break;
           }
       a.ids[row] = id;
@@ -325,168 +466,166 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
     return;
   }
   const bool infinite = largest == INFINITY;
-  const double top = bin_of(infinite ? 0.0 : (double)largest, r.per_t);
-  // how far the first bin of a part lies below the row's
-  const auto behind = [&](int i) {
-    const float m = finite(parts[i].largest, infinite);
-    const double d = top - bin_of((double)m, r.per_t);
-    return m == -INFINITY || d >= kBins ? kBins : (int)d;
-  };
-  const Choose<T> c{s, r, (const T*)a.logits + row * a.ld, s.chunk + row * s.chunks, top, infinite, held, digit, digit_count, words, &count};
+  largest = finite(largest, infinite);
+  const double top = uniform(bin_of(largest, r));
+  const Choose<T> c{s, r, (const T*)a.logits + row * a.ld, s.chunk + row * s.chunks, m, largest, top, infinite};
+  // how far the first bin of a part lies below the row's; its bin i is the row's behind + i
+  if (tid < S) {
+    const float l = finite(m.part[tid].largest, infinite);
+    const double d = top - bin_of(l, r);
+    m.behind[tid] = l == -INFINITY || !(d < kBins) ? kBins : (int)d;
+  }
+  __syncthreads();
   const uint64_t* const histogram = s.histogram + row * S * kBins;
-  // weights, relative to e^((top + 1) / 4), of a part's bin
-  const auto part_bin = [&](int i, int j) { return histogram[(int64_t)i * kBins + place_of(top - j)]; };
-  constexpr uint64_t kSumMask = (1ull << kCountShift) - 1;
-  constexpr double kUnit = 1.0 / (double)(1ll << kFixed);
 
   int end = kBins;          // bins below it are kept whole, those above it not at all
   uint64_t border = 0;      // of bin `end` the tokens that are not behind this in order
   bool at_least = false;    // and those of them that weigh at least min_p
-  const double heaviest = infinite ? 0.0 : (double)largest * r.per_t * 0.25;
+  const double heaviest = uniform((double)largest * r.per_t * 0.25);
   const auto heavy = [&](float l) { return exp((double)l * r.per_t * 0.25 - heaviest) >= (double)r.min_p; };
   if (r.filtered) {
-    if (tid < kBins) {
-      uint64_t sum = 0;
-      uint32_t n = 0;
-      for (int i = 0; i < S; ++i)
-        if (tid >= behind(i)) {
-          const uint64_t h = part_bin(i, tid);
-          sum += h & kSumMask;
-          n += (uint32_t)(h >> kCountShift);
+    for (int i = tid / kBins; i < S; i += kChoose / kBins) {
+      const int j = m.behind[i] + tid % kBins;
+      if (j >= kBins) continue;
+      const uint64_t h = histogram[i * kBins + tid % kBins];
+      if (h == 0) continue;
+      atomicAdd((unsigned long long*)&m.fixed[j], (unsigned long long)(h & kSumMask));
+      atomicAdd(&m.bin_count[j], (uint32_t)(h >> kCountShift));
+    }
+    __syncthreads();
+    double sum[4], all = 0.0;
+    uint32_t count[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sum[i] = (double)m.fixed[4 * lane + i] * kUnit * m.table[4 * lane + i];
+      count[i] = m.bin_count[4 * lane + i];
+      all += sum[i];
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) all += __shfl_xor(all, off, 64);
+    all = uniform(all);
+    uint64_t from = 0, to = 0;  // the orders of bin `end`
+    // top-k, top-p and min-p, each within what those ahead of it keep
+#pragma unroll 1
+    for (int filter = 0; filter < 3; ++filter) {
+      int j;
+      uint32_t need = 0;
+      double reach = 0.0;
+      if (filter < 2) {
+        if (filter == 0 ? r.top_k == 0 : !(r.top_p < 1.0f)) continue;
+        const double target = (double)r.top_p * all;
+        Found<double> f = first_full(sum, count, [&](double su, uint32_t n) { return filter ? su >= target : n >= (uint32_t)r.top_k; });
+        if (f.at == kBins) continue;
+        j = min(f.at, end);
+        if (j < f.at) {  // (a rounding away from all that top-k keeps: the bin that it ends in)
+          f.sum = 0.0;
+          for (int i = 0; i < j; ++i) f.sum += (double)m.fixed[i] * kUnit * m.table[i];
+          f.sum = uniform(f.sum);
         }
-      fixed[tid] = sum;
-      counts[tid] = n;
-    }
-    __syncthreads();
-    // every thread walks the bins; a row's tokens end in one of them
-    double above = 0.0, all = 0.0;
-    for (int j = 0; j < kBins; ++j) all += (double)fixed[j] * kUnit * table[j];
-    if (r.top_k) {
-      uint32_t n = 0;
-      int j = 0;
-      for (; j < kBins && n + counts[j] < (uint32_t)r.top_k; ++j) n += counts[j], above += (double)fixed[j] * kUnit * table[j];
-      if (j < kBins) {
-        end = j;
-        c.gather(j, counts[j]);
-        c.last_kept(j, counts[j], false, r.top_k - n, 0.0);
-        border = words[0];
-        all = above + (double)words[1] * kUnit * table[j];
-      }
-    }
-    if (r.top_p < 1.0f) {
-      const double target = (double)r.top_p * all;
-      double sum = 0.0;
-      int j = 0;
-      for (; j < kBins && j < end; ++j) {
-        const double with = sum + (double)fixed[j] * kUnit * table[j];
-        if (with >= target) break;
-        sum = with;
-      }
-      if (j < kBins && counts[j]) {
-        if (j != end) c.gather(j, counts[j]);
-        c.last_kept(j, counts[j], true, 0, (target - sum) / (kUnit * table[j]));
-        // (nothing reaches it: a rounding away from the whole bin)
-        if (j != end) border = words[0];
-        else if (words[0] > border) border = words[0];
-        end = j;
-      }
-    }
-    if (r.min_p > 0.0f) {
-      const double d = top - floor((heaviest + log((double)r.min_p)) * 4.0);
-      const int j = d >= kBins ? kBins : max((int)d, 0);
-      if (j < end) {
-        end = j;
+        need = r.top_k - f.count;
+        reach = uniform((target - f.sum) / (kUnit * m.table[j]));
+        if (filter == 0) all = f.sum;  // and what is kept of bin j
+      } else {
+        if (!(r.min_p > 0.0f)) continue;
+        const double d = top - floor((heaviest + log((double)r.min_p)) * 4.0);
+        j = uniform(d >= kBins ? kBins : max((int)d, 0));
+        if (j > end || j == kBins) continue;
+        at_least = true;
+        if (j == end) continue;
         border = 0;
-        at_least = true;
-        c.gather(j, counts[j]);
-      } else if (j == end && j < kBins) {
-        at_least = true;
       }
+      const int n = uniform((int)m.bin_count[j]);
+      if (j != end) c.gather(j, n, from, to);
+      if (filter < 2) {
+        c.last_kept(n, from, to, filter == 1, need, reach);
+        const uint64_t last = uniform(m.word[0]);
+        border = j == end && border > last ? border : last;
+        if (filter == 0) all = uniform(all + (double)m.word[1] * kUnit * m.table[j]);
+      }
+      end = j;
     }
-    __syncthreads();
-    if (tid < kMostParts) in_bin[tid] = 0;
     __syncthreads();
     if (end < kBins)
-      c.each(end, counts[end], [&](uint64_t order, uint64_t weight) {
-        if (order >= border && (!at_least || heavy(c.logit_of(order))))
-          atomicAdd((unsigned long long*)&in_bin[(uint32_t)~(uint32_t)order / kPart], (unsigned long long)weight);
+      c.each(uniform((int)m.bin_count[end]), from, to, [&](uint64_t order) {
+        if (order >= border && (!at_least || heavy(logit_of((uint32_t)(order >> 32)))))
+          atomicAdd((unsigned long long*)&m.in_bin[(uint32_t)~(uint32_t)order / kPart], (unsigned long long)c.fixed_at(order));
       });
     __syncthreads();
     for (int i = wave; i < S; i += kChoose / 64) {
-      double sum = 0.0;
-      const int from = behind(i);
-      for (int j = lane; j < end; j += 64)
-        if (j >= from) sum += (double)(part_bin(i, j) & kSumMask) * kUnit * table[j];
+      double part = 0.0;
+      for (int b = lane; b + m.behind[i] < end; b += 64) part += (double)(histogram[i * kBins + b] & kSumMask) * kUnit * m.table[b + m.behind[i]];
 #pragma unroll
-      for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-      if (lane == 0) part_sum[i] = end < kBins ? sum + (double)in_bin[i] * kUnit * table[end] : sum;
+      for (int off = 32; off > 0; off >>= 1) part += __shfl_xor(part, off, 64);
+      if (lane == 0) m.part_sum[i] = end < kBins ? part + (double)m.in_bin[i] * kUnit * m.table[end] : part;
     }
   } else if (tid < S) {
-    const int from = behind(tid);
-    part_sum[tid] = from < kBins ? parts[tid].sum * table[from] : 0.0;
+    m.part_sum[tid] = m.behind[tid] < kBins ? m.part[tid].sum * m.table[m.behind[tid]] : 0.0;
   }
   __syncthreads();
   double total = 0.0;
-  for (int i = 0; i < S; ++i) total += part_sum[i];
+  for (int i = 0; i < S; ++i) total += m.part_sum[i];
   const double target = (double)fminf(fmaxf(a.uniform[row], 0.0f), 0x1.fffffep-1f) * total;
   double base = 0.0;
-  int part = -1;
+  int part = -1;  // (a row has some weight, and so has one of its parts)
   for (int i = 0; i < S; ++i) {
-    if (part_sum[i] <= 0.0) continue;
-    if (part >= 0) base += part_sum[part];
+    if (m.part_sum[i] <= 0.0) continue;
+    if (part >= 0) base += m.part_sum[part];
     part = i;
-    if (base + part_sum[i] > target) break;
+    if (base + m.part_sum[i] > target) break;
   }
+  part = max(part, 0);
   // A uniform number this close to 0 asks for the first tokens, whose weights may be those that the sums do without: part after part.
   const bool least = target < total * 0x1p-60;
   if (least) base = 0.0, part = 0;
+  typedef typename Some<T, kPart / kChoose>::type some_t;
   for (;; ++part) {
-    // eight logits of the part a thread, in order
-    double mine[8], sum = 0.0;
-    const int at = part * kPart + tid * 8;
+    // sixteen logits of the part a thread, in order
+    constexpr int kEach = kPart / kChoose;
+    double mine[kEach], sum = 0.0;
+    const int at = part * kPart + tid * kEach;
+    some_t v;
+    if (at + kEach <= a.vocab) {
+      v = *reinterpret_cast<const some_t*>(c.x + at);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < kEach; ++e) v[e] = at + e < a.vocab ? c.x[at + e] : (T)-INFINITY;
+    }
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
       mine[e] = 0.0;
-      if (at + e < a.vocab) {
-        const float l = c.at(at + e);
-        const Binned b = binned(l, r.per_t);
-        const int j = c.below(b, l);
-        if (j < end || (j == end && j < kBins && order_of(l, at + e) >= border && (!at_least || heavy(l)))) mine[e] = b.weight * table[j];
-        if (least && j == kBins && end == kBins) mine[e] = exp((double)l * r.per_t * 0.25 - heaviest);
-      }
+      const float l = finite(logit((float)v[e]), infinite);
+      const Binned b = binned(l, r);
+      const int j = c.below(b, l);
+      if (j < end || (j == end && j < kBins && order_of(l, at + e) >= border && (!at_least || heavy(l)))) mine[e] = weight_of(b) * m.table[j];
+      if (least && j == kBins && end == kBins) mine[e] = exp((double)l * r.per_t * 0.25 - heaviest);
       sum += mine[e];
     }
-    double before = sum;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const double v = __shfl_up(before, off, 64);
-      if (lane >= off) before += v;
-    }
-    if (lane == 63) wave_sum[wave] = before;
+    double before = sums_of_wave(sum);
+    if (lane == 63) m.wave_sum[wave] = before;
     __syncthreads();
     before = base + (before - sum);
     for (int w = 0; w < kChoose / 64; ++w) {
-      if (w < wave) before += wave_sum[w];
-      base += wave_sum[w];
+      if (w < wave) before += m.wave_sum[w];
+      base += m.wave_sum[w];
     }
     int kept = -1;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < kEach; ++e) {
       if (mine[e] > 0.0) {
         before += mine[e];
         kept = at + e;
         if (before > target) {
-          atomicMin(&pick, at + e);
+          atomicMin(&m.pick, at + e);
           break;
         }
       }
     }
-    if (kept >= 0) atomicMax(&last, kept);
+    if (kept >= 0) atomicMax(&m.last, kept);
     __syncthreads();
-    if (!least || pick != INT32_MAX || part + 1 == S) break;
+    if (!least || m.pick != INT32_MAX || part + 1 == S) break;
     __syncthreads();  // everyone has seen that there is no pick yet
   }
-  if (tid == 0) a.ids[row] = pick == INT32_MAX ? last : pick;  // (a rounding away from the end: the last one kept)
+  if (tid == 0) a.ids[row] = m.pick == INT32_MAX ? m.last : m.pick;  // (a rounding away from the end: the last one kept)
 }
 
 inline int parts_of(int64_t vocab) { return (int)((vocab + kPart - 1) / kPart); }
