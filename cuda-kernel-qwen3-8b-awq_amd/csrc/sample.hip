@@ -4,15 +4,15 @@
 
 namespace {
 
-// Weights go into bins of a quarter of a nat, y = 4 l / T, bin floor(y); of a row or a part of it only the 256 bins from its largest logit's down
-// are looked at: what lies further is below e^-63, and 64 bits of a sum would not show it.  Within a bin a weight is e^((y - bin - 1) / 4),
-// between e^(-1/4) and 1, as a whole multiple of 2^-36, so that sums do not depend on their order; bins are joined in 64-bit floating point.
+// Weights go into bins of an eighth of a nat, y = 8 l / T, bin floor(y); of a row or a part of it only the 512 bins from its largest logit's down
+// are looked at: what lies further is below e^-63, and 64 bits of a sum would not show it.  Within a bin a weight is e^((y - bin - 1) / 8),
+// between e^(-1/8) and 1, as a whole multiple of 2^-36, so that sums do not depend on their order; bins are joined in 64-bit floating point.
 // (Tokens with the largest logit are all in the first bin: their sums are exact, and uniform numbers such as 1/2 fall between two of them as
 // they should.)
 //   scan_kernel    parts of 8,192 logits: largest, sum of weights, and where a row is filtered a histogram, sums and counts by bin
 //   choose_kernel  a workgroup a row: the bin in which the tokens kept end, the order within that bin alone, the part that the uniform
 //                  number falls in, and the token in that part.
-constexpr int kPart = 8192, kScan = 256, kChoose = 512, kBins = 256, kChunk = 32, kHeld = 8192, kFew = 512, kMostParts = 64;
+constexpr int kPart = 8192, kScan = 256, kChoose = 512, kBins = 512, kDigits = 256, kChunk = 32, kHeld = 8192, kFew = 512, kMostParts = 64;
 constexpr int kMostChunks = kMostParts * kPart / kChunk, kCopies = 8;
 constexpr int kFixed = 36, kCountShift = 50;
 constexpr uint64_t kSumMask = (1ull << kCountShift) - 1;
@@ -22,7 +22,7 @@ constexpr double kRound = 0x1.8p16;  // numbers of its size are 2^-36 apart
 struct Part {
   float largest;
   int32_t first;  // lowest id of the largest
-  double sum;     // of the weights, relative to e^((bin + 1) / 4) of the largest's bin
+  double sum;     // of the weights, relative to e^((bin + 1) / 8) of the largest's bin
 };
 struct SampleArgs {
   awq_sample_args a;
@@ -40,8 +40,7 @@ __device__ __forceinline__ uint64_t uniform(uint64_t v) { return (uint64_t)unifo
 __device__ __forceinline__ double uniform(double v) { return __longlong_as_double((long long)uniform((uint64_t)__double_as_longlong(v))); }
 
 struct Row {
-  double per_t;  // 4 / T
-  float limit;   // logits beyond 2^48 T count as that
+  double per_t;  // 8 / T
   float top_p, min_p;
   int top_k;  // 0: not limited
   bool greedy, filtered;
@@ -50,8 +49,7 @@ __device__ __forceinline__ Row row_of(const awq_sample_args& a, int64_t row) {
   Row r;
   const float t = a.temperature ? a.temperature[row] : 1.0f;
   r.greedy = !(t > 0.0f);
-  r.per_t = uniform(4.0 / (double)t);
-  r.limit = fminf(0x1p48f * t, 3.4028234663852886e38f);
+  r.per_t = uniform(8.0 / (double)t);
   r.top_k = a.top_k ? a.top_k[row] : 0;
   if (r.top_k < 0 || r.top_k >= a.vocab) r.top_k = 0;
   r.top_p = a.top_p ? a.top_p[row] : 1.0f;
@@ -63,21 +61,20 @@ __device__ __forceinline__ Row row_of(const awq_sample_args& a, int64_t row) {
   return r;
 }
 
-__device__ __forceinline__ double y_of(float l, const Row& r) { return (double)fminf(fmaxf(l, -r.limit), r.limit) * r.per_t; }
-__device__ __forceinline__ double bin_of(float l, const Row& r) { return floor(y_of(l, r)); }
+__device__ __forceinline__ double bin_of(float l, const Row& r) { return floor((double)l * r.per_t); }
 struct Binned {
-  double bin, rounded;  // rounded: kRound + the weight relative to e^((bin + 1) / 4)
+  double bin, rounded;  // rounded: kRound + the weight relative to e^((bin + 1) / 8)
 };
 __device__ __forceinline__ Binned binned(float l, const Row& r) {
-  const double y = y_of(l, r), b = floor(y), x = y - b;
-  // e^((x - 1) / 4) for x from 0 to 1: the polynomial through its values at the seven Chebyshev points, within 1.7e-12
-  double e = 2.9938727103789073e-07;
-  e = fma(e, x, 6.288293243577365e-06);
-  e = fma(e, x, 0.00012679210980033013);
-  e = fma(e, x, 0.002028115011608631);
-  e = fma(e, x, 0.02433752648211561);
-  e = fma(e, x, 0.1947001956419453);
-  e = fma(e, x, 0.7788007830726902);
+  // (of y beyond 2^53 x is 0, and different logits are too far from each other to meet)
+  const double y = (double)l * r.per_t, b = floor(y), x = y - b;
+  // e^((x - 1) / 8) for x from 0 to 1: the polynomial through its values at the six Chebyshev points, within 2.8e-12
+  double e = 2.389384121670446e-07;
+  e = fma(e, x, 8.96072434860192e-06);
+  e = fma(e, x, 0.0002872797252023532);
+  e = fma(e, x, 0.0068945050309035805);
+  e = fma(e, x, 0.11031211299649428);
+  e = fma(e, x, 0.8824969025821857);
   return {b, e + kRound};
 }
 // the weight as a multiple of 2^-36, and as a number
@@ -110,8 +107,9 @@ __global__ __launch_bounds__(kScan) void scan_kernel(SampleArgs s) {
   __shared__ float largest_of[kScan / 64];
   __shared__ int first_of[kScan / 64];
   __shared__ double sum_of[kScan / 64];
-  __shared__ unsigned long long bins[kBins * kCopies];  // (copies by lane: lanes that meet in a bin wait for each other)
-  __shared__ double table[kBins];
+  // (copies by lane: lanes that meet in a bin wait for each other; a bin behind the last for what is further, which nobody reads)
+  __shared__ unsigned long long bins[(kBins + 1) * kCopies];
+  __shared__ double table[kBins + 1];
   const awq_sample_args& a = s.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x / s.parts;
@@ -124,10 +122,10 @@ __global__ __launch_bounds__(kScan) void scan_kernel(SampleArgs s) {
     if (at + W <= a.vocab) {
       const vec_t u = *reinterpret_cast<const vec_t*>(x + at);
 #pragma unroll
-      for (int e = 0; e < W; ++e) v[i][e] = logit((float)u[e]);
+      for (int e = 0; e < W; ++e) v[i][e] = fmaxf((float)u[e], -INFINITY);  // (of NaN -infinity)
     } else {
 #pragma unroll
-      for (int e = 0; e < W; ++e) v[i][e] = at + e < a.vocab ? logit((float)x[at + e]) : -INFINITY;
+      for (int e = 0; e < W; ++e) v[i][e] = at + e < a.vocab ? fmaxf((float)x[at + e], -INFINITY) : -INFINITY;
     }
   }
   const Row r = row_of(a, row);
@@ -135,7 +133,8 @@ __global__ __launch_bounds__(kScan) void scan_kernel(SampleArgs s) {
     if (r.filtered) {
       for (int b = tid; b < kBins * kCopies; b += kScan) bins[b] = 0;
     } else {
-      table[tid] = exp(-0.25 * tid);
+      for (int b = tid; b < kBins; b += kScan) table[b] = exp(-0.125 * b);
+      if (tid == 0) table[kBins] = 0.0;
     }
   }
   float largest = -INFINITY;
@@ -146,12 +145,12 @@ __global__ __launch_bounds__(kScan) void scan_kernel(SampleArgs s) {
     for (int e = 1; e < W; ++e) m = fmaxf(m, v[i][e]);
     largest = fmaxf(largest, m);
     if (r.filtered) {
-      m = lanes::maximum<LANES>(m);
+      m = lanes::maximum<LANES>(m) + 0.0f;  // (-0 as 0)
       const int64_t at = ((int64_t)part * kPart + (i * kScan + tid) * W) / kChunk;
       if (tid % LANES == 0 && at < s.chunks) s.chunk[row * s.chunks + at] = m;
     }
   }
-  largest = lanes::maximum<64>(largest);
+  largest = lanes::maximum<64>(largest) + 0.0f;
   if (lane == 0) largest_of[wave] = largest;
   __syncthreads();
 #pragma unroll
@@ -171,25 +170,41 @@ __global__ __launch_bounds__(kScan) void scan_kernel(SampleArgs s) {
     out.first = min(min(first_of[0], first_of[1]), min(first_of[2], first_of[3]));
   } else if (largest > -INFINITY) {
     const bool infinite = largest == INFINITY;
+    if (infinite) {
+#pragma unroll
+      for (int i = 0; i < L; ++i)
+#pragma unroll
+        for (int e = 0; e < W; ++e) v[i][e] = finite(v[i][e], true);
+    }
     const double top = bin_of(finite(largest, infinite), r);
+    // (a float as the number of a far bin is the largest of its kind)
+    const auto place = [&](const Binned& b) __attribute__((always_inline)) { return min((uint32_t)__builtin_elementwise_min(top - b.bin, 4e9), (uint32_t)kBins); };
     double sum = 0.0;
+    if (r.filtered) {
 #pragma unroll
-    for (int i = 0; i < L; ++i)
+      for (int i = 0; i < L; ++i)
 #pragma unroll
-      for (int e = 0; e < W; ++e) {
-        const float l = finite(v[i][e], infinite);
-        const Binned b = binned(l, r);
-        const double below = top - b.bin;
-        if (!(below < kBins) || l == -INFINITY) continue;
-        if (r.filtered) atomicAdd(&bins[(int)below * kCopies + lane % kCopies], (1ull << kCountShift) | fixed_of(b));
-        else sum += weight_of(b) * table[(int)below];
-      }
+        for (int e = 0; e < W; ++e) {
+          const Binned b = binned(v[i][e], r);
+          atomicAdd(&bins[place(b) * kCopies + lane % kCopies], (1ull << kCountShift) | fixed_of(b));
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < L; ++i)
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          const Binned b = binned(v[i][e], r);
+          sum = fma(fmax(weight_of(b), 0.0), table[place(b)], sum);  // (of -infinity NaN)
+        }
+    }
     if (r.filtered) {
       __syncthreads();
-      unsigned long long all = 0;
+      for (int b = tid; b < kBins; b += kScan) {
+        unsigned long long all = 0;
 #pragma unroll
-      for (int c = 0; c < kCopies; ++c) all += bins[tid * kCopies + (c + tid) % kCopies];
-      s.histogram[(row * s.parts + part) * kBins + tid] = all;
+        for (int c = 0; c < kCopies; ++c) all += bins[b * kCopies + (c + tid) % kCopies];
+        s.histogram[(row * s.parts + part) * kBins + b] = all;
+      }
     } else {
 #pragma unroll
       for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
@@ -205,12 +220,12 @@ struct ChooseMemory {
   uint64_t held[kHeld];       // order of the tokens of a bin, where they are so few
   uint16_t list[kMostChunks]; // chunks that have some
   uint64_t few[kFew], few_weight[kFew];
-  uint64_t digit[kBins];
-  uint32_t digit_count[kBins];
+  uint64_t digit[kDigits];
+  uint32_t digit_count[kDigits];
   uint64_t word[2], in_bin[kMostParts];
   uint64_t fixed[kBins];
   uint32_t bin_count[kBins];
-  double table[kBins], part_sum[kMostParts], wave_sum[kChoose / 64];
+  double table[kBins], part_sum[kMostParts], wave_sum[kChoose / 64], until[kChoose];
   Part part[kMostParts];
   int behind[kMostParts];
   uint32_t held_count, list_count, few_count;
@@ -228,7 +243,7 @@ __device__ __forceinline__ T sums_of_wave(T v) {
   return v;
 }
 
-// The first of 256 entries, four a lane, at which `full` holds of the sums up to it (itself included), and the sums ahead of it; 256: none.
+// The first of 64 N entries, N a lane, at which `full` holds of the sums up to it (itself included), and the sums ahead of it; 64 N: none.
 // Every wavefront finds it for itself.
 template <typename S>
 struct Found {
@@ -236,33 +251,32 @@ struct Found {
   S sum;
   uint32_t count;
 };
-template <typename S, typename F>
-__device__ __forceinline__ Found<S> first_full(const S (&sum)[4], const uint32_t (&count)[4], F full) {
+template <int N, typename S, typename F>
+__device__ __forceinline__ Found<S> first_full(const S (&sum)[N], const uint32_t (&count)[N], F full) {
   const int lane = threadIdx.x & 63;
-  const S mine = ((sum[0] + sum[1]) + sum[2]) + sum[3];
-  const uint32_t many = count[0] + count[1] + count[2] + count[3];
-  S s = sums_of_wave(mine) - mine;
-  if constexpr (__is_same(S, double)) {  // (the sums ahead as they are formed, not as a difference)
-    const S up = __shfl_up(sums_of_wave(mine), 1, 64);
-    s = lane ? up : 0.0;
-  }
+  S mine = sum[0];
+  uint32_t many = count[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) mine += sum[i], many += count[i];
+  const S up = __shfl_up(sums_of_wave(mine), 1, 64);  // (the sums ahead as they are formed, not as a difference)
+  S s = lane ? up : (S)0;
   uint32_t n = sums_of_wave(many) - many;
-  int at = 4;
+  int at = N;
   S before = s;
   uint32_t before_count = n;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < N; ++i) {
     s += sum[i];
     n += count[i];
-    if (at == 4) {
+    if (at == N) {
       if (full(s, n)) at = i;
       else before = s, before_count = n;
     }
   }
-  const unsigned long long any = __builtin_amdgcn_ballot_w64(at < 4);
-  if (any == 0) return {kBins, (S)0, 0};
+  const unsigned long long any = __builtin_amdgcn_ballot_w64(at < N);
+  if (any == 0) return {64 * N, (S)0, 0};
   const int from = __builtin_ctzll(any);
-  return {uniform(4 * from + __shfl(at, from, 64)), uniform(__shfl(before, from, 64)), uniform((uint32_t)__shfl((int)before_count, from, 64))};
+  return {uniform(N * from + __shfl(at, from, 64)), uniform(__shfl(before, from, 64)), uniform((uint32_t)__shfl((int)before_count, from, 64))};
 }
 
 template <typename T>
@@ -277,7 +291,7 @@ struct Choose {
   bool infinite;
 
   __device__ __forceinline__ float at(int i) const { return finite(logit((float)x[i]), infinite); }
-  // distance of a logit's bin from the row's first; 256: further or no weight
+  // distance of a logit's bin from the row's first; kBins: further or no weight
   __device__ __forceinline__ int below(const Binned& b, float l) const {
     const double d = top - b.bin;
     return l == -INFINITY || !(d < kBins) ? kBins : (int)d;
@@ -294,31 +308,46 @@ struct Choose {
     }
     return hi;
   }
-  // every token of the orders a .. b - 1: f(order); out of the row, by the chunks listed, 16 bytes of a chunk a thread and four of them at once
-  template <typename F>
-  __device__ __forceinline__ void each_of_row(uint64_t a, uint64_t b, F f) const {
+  // the tokens of the orders a .. b - 1 into `held`, out of the row, by the chunks listed: 16 bytes of a chunk a thread and four of them at once
+  __device__ __forceinline__ void hold(uint64_t a, uint64_t b) const {
     constexpr int W = 16 / sizeof(T), LANES = kChunk / W, AT_ONCE = kChoose / LANES, U = 4;
     typedef typename Some<T, W>::type vec_t;
     const int vocab = (int)s.a.vocab, n = uniform((int)m.list_count), first = threadIdx.x / LANES, in_chunk = threadIdx.x % LANES * W;
-    for (int c0 = first; c0 < n; c0 += U * AT_ONCE) {
+    const uint32_t low = (uint32_t)(a >> 32), high = (uint32_t)(b >> 32);  // (of keys: a and b are whole keys)
+    for (int c0 = 0; c0 < n; c0 += U * AT_ONCE) {
       vec_t v[U];
       int id[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        id[u] = c0 + u * AT_ONCE < n ? m.list[c0 + u * AT_ONCE] * kChunk + in_chunk : vocab;
-        if (id[u] + W <= vocab) v[u] = *reinterpret_cast<const vec_t*>(x + id[u]);
-      }
+        const int c = c0 + u * AT_ONCE + first;
+        id[u] = c < n ? m.list[c] * kChunk + in_chunk : vocab;
+        if (id[u] + W <= vocab) {
+          v[u] = *reinterpret_cast<const vec_t*>(x + id[u]);
+        } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (id[u] >= vocab) continue;
-#pragma unroll
-        for (int e = 0; e < W; ++e) {
-          if (id[u] + W > vocab && id[u] + e >= vocab) continue;
-          const float l = finite(logit(id[u] + W <= vocab ? (float)v[u][e] : (float)x[id[u] + e]), infinite);
-          const uint64_t order = order_of(l, id[u] + e);
-          if (order >= a && order < b) f(order);
+          for (int e = 0; e < W; ++e) v[u][e] = id[u] + e < vocab ? x[id[u] + e] : (T)-INFINITY;
         }
       }
+      uint32_t in = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          const uint32_t key = key_of(finite(logit((float)v[u][e]), infinite));
+          in |= (uint32_t)(key >= low && key < high) << (u * W + e);
+        }
+      const uint32_t mine = __builtin_popcount(in), upto = sums_of_wave(mine);
+      uint32_t to = 0;
+      if ((threadIdx.x & 63) == 63 && upto) to = atomicAdd(&m.held_count, upto);
+      to = (uint32_t)__builtin_amdgcn_readlane((int)to, 63) + upto - mine;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+          if (in >> (u * W + e) & 1) {
+            if (to < (uint32_t)kHeld) m.held[to] = order_of(finite(logit((float)v[u][e]), infinite), id[u] + e);
+            ++to;
+          }
     }
   }
   __device__ __forceinline__ uint64_t fixed_at(uint64_t order) const { return fixed_of(binned(logit_of((uint32_t)(order >> 32)), r)); }
@@ -347,22 +376,28 @@ struct Choose {
     if (threadIdx.x == 0) m.held_count = m.list_count = 0;
     __syncthreads();
     const int lane = threadIdx.x & 63;
-    for (int c0 = 0; c0 < s.chunks; c0 += kChoose) {
-      const int c = c0 + threadIdx.x;
-      const bool some = c < s.chunks && key_of(finite(chunk[min(c, s.chunks - 1)], infinite)) >= low;
-      const unsigned long long any = __builtin_amdgcn_ballot_w64(some);
-      if (any == 0) continue;
-      uint32_t to = 0;
-      if (lane == 0) to = atomicAdd(&m.list_count, (uint32_t)__builtin_popcountll(any));
-      to = __builtin_amdgcn_readfirstlane(to) + __builtin_popcountll(any & ((1ull << lane) - 1));
-      if (some) m.list[to] = (uint16_t)c;
+    constexpr int U = 4;
+    for (int c0 = 0; c0 < s.chunks; c0 += U * kChoose) {
+      float largest_of[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int c = c0 + u * kChoose + threadIdx.x;
+        largest_of[u] = c < s.chunks ? chunk[c] : -INFINITY;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool some = key_of(finite(largest_of[u], infinite)) >= low;
+        const unsigned long long any = __builtin_amdgcn_ballot_w64(some);
+        if (any == 0) continue;
+        uint32_t to = 0;
+        if (lane == 0) to = atomicAdd(&m.list_count, (uint32_t)__builtin_popcountll(any));
+        to = uniform(to) + __builtin_popcountll(any & ((1ull << lane) - 1));
+        if (some) m.list[to] = (uint16_t)(c0 + u * kChoose + threadIdx.x);
+      }
     }
     __syncthreads();
     if (n > kHeld) return;
-    each_of_row(a, b, [&](uint64_t order) {
-      const uint32_t to = atomicAdd(&m.held_count, 1u);
-      if (to < (uint32_t)kHeld) m.held[to] = order;
-    });
+    hold(a, b);
     __syncthreads();
   }
   // Of a bin's n tokens, of the orders a .. b - 1, the one with which the count (by_sum == false: `need` of them) or the sum of the weights (the first at
@@ -377,7 +412,7 @@ struct Choose {
     while (n > kFew) {
       const int shift = max(0, 56 - __builtin_clzll(b - a - 1));  // (b - a - 1) >> shift is below 256
       __syncthreads();
-      if (tid < kBins) m.digit[tid] = 0, m.digit_count[tid] = 0;
+      if (tid < kDigits) m.digit[tid] = 0, m.digit_count[tid] = 0;
       __syncthreads();
       each(all, a, b, [&](uint64_t order) {
         const int d = (int)((order - a) >> shift);
@@ -392,7 +427,7 @@ struct Choose {
       const Found<uint64_t> f = first_full(sum, count, [&](uint64_t su, uint32_t co) {
         return by_sum ? (double)(ahead + su) >= reach : ahead_count + co >= need;
       });
-      if (f.at == kBins) return;  // (a rounding away from all of them)
+      if (f.at == kDigits) return;  // (a rounding away from all of them)
       const uint64_t d = 255 - f.at;
       ahead += f.sum;
       ahead_count += f.count;
@@ -441,8 +476,9 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
   const int64_t row = blockIdx.x;
   if (tid < S) m.part[tid] = s.part[row * S + tid];
   const Row r = row_of(a, row);
+  static_assert(kBins <= kChoose, "a thread a bin");
   if (!r.greedy && tid < kBins) {
-    m.table[tid] = exp(-0.25 * tid);
+    m.table[tid] = exp(-0.125 * tid);
     m.fixed[tid] = 0;
     m.bin_count[tid] = 0;
   }
@@ -481,8 +517,8 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
   int end = kBins;          // bins below it are kept whole, those above it not at all
   uint64_t border = 0;      // of bin `end` the tokens that are not behind this in order
   bool at_least = false;    // and those of them that weigh at least min_p
-  const double heaviest = uniform((double)largest * r.per_t * 0.25);
-  const auto heavy = [&](float l) { return exp((double)l * r.per_t * 0.25 - heaviest) >= (double)r.min_p; };
+  const double heaviest = uniform((double)largest * r.per_t * 0.125);
+  const auto heavy = [&](float l) { return exp((double)l * r.per_t * 0.125 - heaviest) >= (double)r.min_p; };
   if (r.filtered) {
     for (int i = tid / kBins; i < S; i += kChoose / kBins) {
       const int j = m.behind[i] + tid % kBins;
@@ -493,12 +529,13 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
       atomicAdd(&m.bin_count[j], (uint32_t)(h >> kCountShift));
     }
     __syncthreads();
-    double sum[4], all = 0.0;
-    uint32_t count[4];
+    constexpr int N = kBins / 64;
+    double sum[N], all = 0.0;
+    uint32_t count[N];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sum[i] = (double)m.fixed[4 * lane + i] * kUnit * m.table[4 * lane + i];
-      count[i] = m.bin_count[4 * lane + i];
+    for (int i = 0; i < N; ++i) {
+      sum[i] = (double)m.fixed[N * lane + i] * kUnit * m.table[N * lane + i];
+      count[i] = m.bin_count[N * lane + i];
       all += sum[i];
     }
 #pragma unroll
@@ -527,7 +564,7 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
         if (filter == 0) all = f.sum;  // and what is kept of bin j
       } else {
         if (!(r.min_p > 0.0f)) continue;
-        const double d = top - floor((heaviest + log((double)r.min_p)) * 4.0);
+        const double d = top - floor((heaviest + log((double)r.min_p)) * 8.0);
         j = uniform(d >= kBins ? kBins : max((int)d, 0));
         if (j > end || j == kBins) continue;
         at_least = true;
@@ -577,55 +614,47 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
   // A uniform number this close to 0 asks for the first tokens, whose weights may be those that the sums do without: part after part.
   const bool least = target < total * 0x1p-60;
   if (least) base = 0.0, part = 0;
-  typedef typename Some<T, kPart / kChoose>::type some_t;
+  const auto weight_at = [&](int id) __attribute__((always_inline)) {
+    const float l = c.at(id);
+    const Binned b = binned(l, r);
+    const int j = c.below(b, l);
+    if (j < end || (j == end && j < kBins && order_of(l, id) >= border && (!at_least || heavy(l)))) return weight_of(b) * m.table[j];
+    return least && j == kBins && end == kBins ? exp((double)l * r.per_t * 0.125 - heaviest) : 0.0;
+  };
+  constexpr int kEach = kPart / kChoose;
   for (;; ++part) {
-    // sixteen logits of the part a thread, in order
-    constexpr int kEach = kPart / kChoose;
-    double mine[kEach], sum = 0.0;
+    // sixteen logits of the part a thread, in order; then those of the thread that the number falls in, one a lane
+    double sum = 0.0;
     const int at = part * kPart + tid * kEach;
-    some_t v;
-    if (at + kEach <= a.vocab) {
-      v = *reinterpret_cast<const some_t*>(c.x + at);
-    } else {
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) v[e] = at + e < a.vocab ? c.x[at + e] : (T)-INFINITY;
-    }
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      mine[e] = 0.0;
-      const float l = finite(logit((float)v[e]), infinite);
-      const Binned b = binned(l, r);
-      const int j = c.below(b, l);
-      if (j < end || (j == end && j < kBins && order_of(l, at + e) >= border && (!at_least || heavy(l)))) mine[e] = weight_of(b) * m.table[j];
-      if (least && j == kBins && end == kBins) mine[e] = exp((double)l * r.per_t * 0.25 - heaviest);
-      sum += mine[e];
-    }
+#pragma unroll 4
+    for (int e = 0; e < kEach; ++e) sum += at + e < a.vocab ? weight_at(at + e) : 0.0;
     double before = sums_of_wave(sum);
     if (lane == 63) m.wave_sum[wave] = before;
     __syncthreads();
-    before = base + (before - sum);
+    before += base;
+#pragma unroll
     for (int w = 0; w < kChoose / 64; ++w) {
       if (w < wave) before += m.wave_sum[w];
       base += m.wave_sum[w];
     }
-    int kept = -1;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      if (mine[e] > 0.0) {
-        before += mine[e];
-        kept = at + e;
-        if (before > target) {
-          atomicMin(&m.pick, at + e);
-          break;
-        }
-      }
+    if (sum > 0.0) {
+      atomicMax(&m.last, tid);  // (of the last part that is looked at)
+      if (before > target) atomicMin(&m.pick, tid);
     }
-    if (kept >= 0) atomicMax(&m.last, kept);
+    if (tid < kChoose) m.until[tid] = before - sum;
     __syncthreads();
     if (!least || m.pick != INT32_MAX || part + 1 == S) break;
     __syncthreads();  // everyone has seen that there is no pick yet
   }
-  if (tid == 0) a.ids[row] = m.pick == INT32_MAX ? m.last : m.pick;  // (a rounding away from the end: the last one kept)
+  if (wave == 0) {
+    const int thread = m.pick == INT32_MAX ? m.last : m.pick, id = part * kPart + thread * kEach + lane;
+    const double w = lane < kEach && id < a.vocab ? weight_at(id) : 0.0;
+    const double before = m.until[thread] + sums_of_wave(w);
+    const unsigned long long over = __builtin_amdgcn_ballot_w64(w > 0.0 && before > target), some = __builtin_amdgcn_ballot_w64(w > 0.0);
+    // (a rounding away from the end: the last one kept)
+    const int of_thread = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : 0;
+    if (lane == 0) a.ids[row] = part * kPart + thread * kEach + of_thread;
+  }
 }
 
 inline int parts_of(int64_t vocab) { return (int)((vocab + kPart - 1) / kPart); }
