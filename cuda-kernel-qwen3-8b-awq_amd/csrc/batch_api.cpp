@@ -110,6 +110,7 @@ extern "C" int awq_paged_attention(const awq_paged_attention_args* a, int32_t dt
   AWQ_REQUIRE(sixteen_bits(dtype), "bfloat16 or binary16 only");
   AWQ_REQUIRE(paged_shape(a->n_requests, a->heads, a->kv_heads, a->dim, a->max_pages) && page_count(a->n_pages),
               "heads of 64, 128 or 256, a multiple of kv_heads of them; requests and pages in range");
+  AWQ_REQUIRE(isfinite(a->scale), "scale is a number");
   if (a->n_requests == 0) return AWQ_OK;
   AWQ_REQUIRE(a->q && a->ctx && a->lengths && a->workspace, "NULL pointer");
   AWQ_REQUIRE((a->cache && a->table) || a->max_pages == 0, "NULL pointer");
@@ -124,6 +125,7 @@ extern "C" int awq_packed_attention(const awq_packed_attention_args* a, int32_t 
   AWQ_REQUIRE(sixteen_bits(dtype), "bfloat16 or binary16 only");
   AWQ_REQUIRE(cache_heads(a->kv_heads, a->dim) && query_heads(a->heads, a->kv_heads), "heads of 64, 128 or 256, a multiple of kv_heads of them");
   AWQ_REQUIRE(a->n_requests >= 0 && a->n_tokens >= 0 && a->n_tokens < (1ll << 31) && a->n_keys >= 0 && a->n_keys < (1ll << 31), "requests or rows out of range");
+  AWQ_REQUIRE(isfinite(a->scale), "scale is a number");
   AWQ_REQUIRE(a->k_starts || a->n_keys >= a->n_tokens, "keys without starts of their own have the queries'");
   if (a->n_requests == 0 || a->n_tokens == 0) return AWQ_OK;
   AWQ_REQUIRE(a->q && a->ctx && a->q_starts && ((a->k && a->v) || a->n_keys == 0), "NULL pointer");

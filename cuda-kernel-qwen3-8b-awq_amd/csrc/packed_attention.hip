@@ -2,6 +2,8 @@
 #include "batch.hpp"
 #include "tile_halves.hpp"
 
+#include <type_traits>
+
 namespace {
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
@@ -19,17 +21,7 @@ __device__ __forceinline__ f32x16_t product(Vec<half_t>::eight a, Vec<half_t>::e
 __device__ __forceinline__ f32x16_t product(Vec<bf16_t>::eight a, Vec<bf16_t>::eight b, f32x16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
-// any of eight 16-bit numbers infinite or NaN
-template <typename T>
-__device__ __forceinline__ bool not_finite(u32x4_t v) {
-  constexpr uint32_t e = __is_same(T, half_t) ? 0x7c00u : 0x7f80u;
-  bool any = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) any |= (v[i] & e) == e || (v[i] >> 16 & e) == e;
-  return any;
-}
-
-constexpr int kQueries = 128, kKeys = 32;
+constexpr int kQueries = 128;
 
 // The tile of queries a workgroup takes: request r has ceil(queries / 128) of them, tiles are numbered one request behind the other. Every
 // wavefront looks its own up, 64 requests at a time.  False: there are fewer tiles.
@@ -68,20 +60,39 @@ __device__ __forceinline__ bool find_tile(const awq_packed_attention_args& a, in
   return false;
 }
 
-// 128 queries of one head a workgroup, 32 a wavefront; 64 keys and values at a time go through LDS.  Queries are columns throughout, lane
-// (n, kh) = (lane % 32, lane / 32):
+// 0 in place of those that are not finite, and whether there are any
+template <typename T>
+__device__ __forceinline__ u32x4_t only_finite(u32x4_t v, bool& any) {
+  constexpr uint32_t e = __is_same(T, half_t) ? 0x7c00u : 0x7f80u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool low = (v[i] & e) == e, high = (v[i] >> 16 & e) == e;
+    any |= low | high;
+    v[i] &= (low ? 0xffff0000u : 0xffffffffu) & (high ? 0x0000ffffu : 0xffffffffu);
+  }
+  return v;
+}
+
+constexpr int kStep = 64;  // keys
+
+// 128 queries of one head a workgroup, 32 a wavefront; 64 keys and values at a time come into LDS by themselves, the next ones while these are
+// multiplied.  Queries are columns throughout, lane (n, kh) = (lane % 32, lane / 32):
 //     S^T[key][query] = K Q^T,   O^T[c][query] += V^T P^T      v_mfma_f32_32x32x16
 // so that a query's maximum, sum and rescaling stay in a lane and its partner, and the weights a lane forms are the elements it
 // supplies to the second product (slice j: keys 16 j + 8 (e / 4) + 4 kh + e % 4; V^T by the transposing LDS read).  Scores, maxima and sums
-// are binary32; a weight is rounded to the activations' type for the second product, the sum of the weights is that of the rounded ones.
-// Values that are not finite where some query of the tile does not see them are kept out of the product, in which 0 times them is NaN.
+// are binary32; a weight is rounded to the activations' type for the second product alone.
+// A row's 16-byte pieces lie rotated in LDS so that the rows that lanes read together are in all banks.
+// Where some query of the wavefront does not see all keys of a step, values that are not finite are kept out of the product, in which 0 times
+// them is NaN, and are added for the queries that see them.
 template <typename T, int D>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_kernel(awq_packed_attention_args a) {
   typedef typename Vec<T>::eight eight_t;
   typedef typename Vec<T>::four four_t;
-  constexpr int KS = D + 8, VS = D + 16, P = D / 32;  // strides in LDS; 16-byte pieces of 64 keys a thread
-  __shared__ __attribute__((aligned(16))) T tiles[2 * kKeys * (KS + VS)];
-  T *const ks = tiles, *const vs = tiles + 2 * kKeys * KS;
+  typedef __attribute__((address_space(1))) const void* gptr_t;
+  typedef __attribute__((address_space(3))) void* lptr_t;
+  constexpr int PIECES = D / 8, P = D / 32;  // of a row; requests of a wavefront for 64 keys
+  constexpr int kTile = kStep * D;
+  __shared__ __attribute__((aligned(16))) T tiles[4 * kTile];  // keys, values, keys, values
   const int group = a.heads / a.kv_heads;
   const int g = blockIdx.x % a.kv_heads, h = g * group + blockIdx.x / a.kv_heads % group;
   Tile t;
@@ -94,114 +105,144 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_kernel(awq_packe
   const int seen = seen_by(qc);
   const int least = seen_by(min(t.first + wave * 32, nq - 1)), most = seen_by(min(t.first + wave * 32 + 31, nq - 1));
   const int end = seen_by(min(t.first + kQueries - 1, nq - 1));
-  const T* const q = (const T*)a.q + (int64_t)(t.q_begin + qc) * a.ldq + (int64_t)h * D;
   const T* const kg = (const T*)a.k + (int64_t)t.k_begin * a.ldk + (int64_t)g * D;
   const T* const vg = (const T*)a.v + (int64_t)t.k_begin * a.ldv + (int64_t)g * D;
-  eight_t qop[D / 16];
+
+  // rotations of a row's pieces
+  const auto key_turn = [](int row) { return D == 64 ? (row >> 1) & 7 : row & 15; };
+  const auto value_turn = [](int row) { return D == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1; };
+  const auto request = [&](int k0, T* tile) __attribute__((always_inline)) {
+    const int last = end - 1 - k0;  // rows behind it are masked, and are that one again
+    const T* const kp = kg + (int64_t)k0 * a.ldk;
+    const T* const vp = vg + (int64_t)k0 * a.ldv;
 #pragma unroll
-  for (int s = 0; s < D / 16; ++s) qop[s] = *reinterpret_cast<const eight_t*>(q + 16 * s + 8 * kh);
+    for (int i = 0; i < P; ++i) {
+      const int x = 64 * (4 * i + wave) + lane, row = x / PIECES, part = x % PIECES, from = min(row, last);
+      __builtin_amdgcn_global_load_lds((gptr_t)(kp + (int64_t)from * a.ldk + (part ^ key_turn(row)) * 8), (lptr_t)(tile + (4 * i + wave) * 512), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gptr_t)(vp + (int64_t)from * a.ldv + (part ^ value_turn(row)) * 8), (lptr_t)(tile + kTile + (4 * i + wave) * 512), 16, 0, 0);
+    }
+  };
+  if (end > 0) request(0, tiles);
+  eight_t qop[D / 16];
+  {
+    const T* const q = (const T*)a.q + (int64_t)(t.q_begin + qc) * a.ldq + (int64_t)h * D;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      qop[s] = *reinterpret_cast<const eight_t*>(q + 16 * s + 8 * kh);
+      if (a.scale < 0.0f) {  // (the largest score is that of the largest product then)
+        u32x4_t x = __builtin_bit_cast(u32x4_t, qop[s]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] ^= 0x80008000u;
+        qop[s] = __builtin_bit_cast(eight_t, x);
+      }
+    }
+  }
   f32x16_t o[D / 32];
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-  float m_run = -INFINITY, l_run = 0.0f;
-  const float mul = a.scale * 1.44269504088896340736f;
+  float m_run = -INFINITY, l_run = 0.0f;  // (of this lane's keys alone)
+  const float mul = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 0x1p-126f);  // (0 times -infinity would be NaN)
 
-  u32x4_t kr[P], vr[P];
-  const auto load = [&](int k0) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const int pc = tid + i * 256, key = k0 + pc / (D / 8), at = (pc % (D / 8)) * 8;
-      kr[i] = vr[i] = u32x4_t{0, 0, 0, 0};
-      if (key < end) {
-        kr[i] = *reinterpret_cast<const u32x4_t*>(kg + (int64_t)key * a.ldk + at);
-        vr[i] = *reinterpret_cast<const u32x4_t*>(vg + (int64_t)key * a.ldv + at);
-      }
-    }
-  };
-  const auto step = [&](int k0, int half, bool strange) __attribute__((always_inline)) {
-    if (k0 >= most) return;
-    const T* const klane = ks + (half * kKeys + n) * KS + 8 * kh;
+  const auto step = [&](int k0, const T* ks, auto MASKED) __attribute__((always_inline)) {
+    constexpr bool masked = decltype(MASKED)::value;
+    const T* const vs = ks + kTile;
     const int L16 = lane & 15;
-    const T* const vlane = vs + (half * kKeys + 4 * kh + (L16 >> 2)) * VS + 16 * ((lane >> 4) & 1) + 4 * (L16 & 3);
+    // keys 16 j + 4 kh + L16 / 4 and 8 further, components 32 d + 16 ((lane / 16) % 2) + 4 (L16 % 4) .. + 3
     const auto values = [&](int j, int d) __attribute__((always_inline)) {
-      const T* const vp = vlane + 16 * j * VS + d * 32;
-      const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4_t __attribute__((address_space(3)))*)vp);
-      const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4_t __attribute__((address_space(3)))*)(vp + 8 * VS));
+      const int row = 16 * j + 4 * kh + (L16 >> 2), piece = 4 * d + 2 * ((lane >> 4) & 1) + ((L16 >> 1) & 1);
+      const T* const lp = vs + row * D + (piece ^ value_turn(row)) * 8 + (L16 & 1) * 4;
+      const T* const up = vs + (row + 8) * D + (piece ^ value_turn(row + 8)) * 8 + (L16 & 1) * 4;
+      const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4_t __attribute__((address_space(3)))*)lp);
+      const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4_t __attribute__((address_space(3)))*)up);
       const four_t l4 = __builtin_bit_cast(four_t, lo), u4 = __builtin_bit_cast(four_t, hi);
       return eight_t{l4[0], l4[1], l4[2], l4[3], u4[0], u4[1], u4[2], u4[3]};
     };
-    f32x16_t s;
+    f32x16_t s[2];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+    for (int half = 0; half < 2; ++half)
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) s = product(*reinterpret_cast<const eight_t*>(klane + 16 * d), qop[d], s);
-    // s[i]: key k0 + 8 (i / 4) + 4 kh + i % 4
+      for (int i = 0; i < 16; ++i) s[half][i] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] *= mul;
-    if (k0 + kKeys > least) {
+    for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = k0 + 8 * (i >> 2) + 4 * kh + (i & 3) < seen ? s[i] : -INFINITY;
+      for (int half = 0; half < 2; ++half) {
+        const int row = 32 * half + n;
+        s[half] = product(*reinterpret_cast<const eight_t*>(ks + row * D + ((2 * d + kh) ^ key_turn(row)) * 8), qop[d], s[half]);
+      }
+    // s[half][i]: key k0 + 32 half + 8 (i / 4) + 4 kh + i % 4
+    if constexpr (masked) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[half][i] = k0 + 32 * half + 8 * (i >> 2) + 4 * kh + (i & 3) < seen ? s[half][i] : -INFINITY;
     }
-    float mx = s[0];
+    float mx = s[0][0];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[half][i]);
     const HalfPair best = half_pair(mx);
-    move_maximum<false>(fmaxf(best.low, best.high), m_run, l_run, o);
-    const float from = m_run == -INFINITY ? 0.0f : m_run;  // (no key seen yet: all weights are 0)
-    float rs = 0.0f;
-    eight_t pop[2];
+    mx = fmaxf(best.low, best.high);
+    // (the scale goes into the exponent's multiply-add, whose product is exact where the maximum's is rounded: far from zero it is put on ahead)
+    float scale = mul;
+    if (__builtin_amdgcn_ballot_w64(fabsf(mx) * mul > 65536.0f && mx > -INFINITY)) {
+      scale = 1.0f;
+      mx *= mul;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const T p = (T)__builtin_amdgcn_exp2f(s[i] - from);
-      rs += (float)p;
-      pop[i >> 3][i & 7] = p;
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[half][i] *= mul;
     }
-    const HalfPair sums = half_pair(rs);
-    l_run += sums.low + sums.high;
-    if (!strange) {
+    move_maximum<true>(mx > -INFINITY ? mx * scale : -INFINITY, m_run, l_run, o);
+    const float from = m_run == -INFINITY ? 0.0f : m_run;  // (no key seen yet: all weights are 0)
+    eight_t pop[4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) o[d] = product(values(j, d), pop[j], o[d]);
-    } else {  // key by key, from memory
+    for (int half = 0; half < 2; ++half)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const HalfPair p = half_pair((float)pop[i >> 3][i & 7]);
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[half][i], scale, -from));
+        l_run += p;
+        pop[2 * half + (i >> 3)][i & 7] = (T)p;
+      }
+    bool strange = false;
 #pragma unroll
-        for (int both = 0; both < 2; ++both) {
-          const int key = k0 + 8 * (i >> 2) + 4 * both + (i & 3);
-          if (key >= seen) continue;
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) {
+        eight_t v = values(j, d);
+        if constexpr (masked) v = __builtin_bit_cast(eight_t, only_finite<T>(__builtin_bit_cast(u32x4_t, v), strange));
+        o[d] = product(v, pop[j], o[d]);
+      }
+    if constexpr (masked) {
+      if (__builtin_amdgcn_ballot_w64(strange)) {
+#pragma unroll 1
+        for (int key = k0; key < min(k0 + kStep, most); ++key) {
           const T* const v = vg + (int64_t)key * a.ldv + 4 * kh;
-          const float w = both ? p.high : p.low;
 #pragma unroll
           for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-            for (int c = 0; c < 16; ++c) o[d][c] = __builtin_fmaf(w, (float)v[32 * d + 8 * (c >> 2) + (c & 3)], o[d][c]);
+            for (int c = 0; c < 16; ++c) {
+              const float x = (float)v[32 * d + 8 * (c >> 2) + (c & 3)];
+              if (key < seen && !(fabsf(x) < INFINITY)) o[d][c] += x;
+            }
         }
       }
     }
   };
-  const int unmasked = seen_by(min(t.first, nq - 1));  // keys that all queries of the tile see
-  load(0);
-  for (int k0 = 0; k0 < end; k0 += 2 * kKeys) {
-    __syncthreads();  // the last tile's readers are done
-    bool strange = false;
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const int pc = tid + i * 256, key = pc / (D / 8), at = (pc % (D / 8)) * 8;
-      *reinterpret_cast<u32x4_t*>(ks + key * KS + at) = kr[i];
-      *reinterpret_cast<u32x4_t*>(vs + key * VS + at) = vr[i];
-      if (k0 + 2 * kKeys > unmasked) strange |= not_finite<T>(vr[i]);
-    }
-    strange = __syncthreads_or(strange) != 0;
-    load(k0 + 2 * kKeys);
-    step(k0, 0, strange);
-    step(k0 + kKeys, 1, strange);
+  T* ks = tiles;
+  for (int k0 = 0; k0 < end; k0 += kStep) {
+    __syncthreads();  // these keys and values are there, the last ones' readers done
+    T* const other = tiles + (ks == tiles ? 2 * kTile : 0);
+    if (k0 + kStep < end) request(k0 + kStep, other);
+    if (k0 + kStep <= least) step(k0, ks, std::false_type());
+    else if (k0 < most) step(k0, ks, std::true_type());
+    ks = other;
   }
   if (qi >= nq) return;
-  const float inv = l_run != 0.0f ? 1.0f / l_run : 0.0f;
+  const HalfPair sums = half_pair(l_run);
+  const float l = sums.low + sums.high, inv = l != 0.0f ? 1.0f / l : 0.0f;
   T* const out = (T*)a.ctx + (int64_t)(t.q_begin + qi) * a.ldc + (int64_t)h * D;
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)

@@ -308,46 +308,46 @@ struct Choose {
     }
     return hi;
   }
-  // the tokens of the orders a .. b - 1 into `held`, out of the row, by the chunks listed: 16 bytes of a chunk a thread and four of them at once
+  // the tokens of the orders a .. b - 1 into `held`, out of the row, by the chunks listed: 16 bytes of a chunk a thread and four of them at once.
+  // First their ids, which a few lanes have at a time; then a logit a thread.
   __device__ __forceinline__ void hold(uint64_t a, uint64_t b) const {
     constexpr int W = 16 / sizeof(T), LANES = kChunk / W, AT_ONCE = kChoose / LANES, U = 4;
     typedef typename Some<T, W>::type vec_t;
     const int vocab = (int)s.a.vocab, n = uniform((int)m.list_count), first = threadIdx.x / LANES, in_chunk = threadIdx.x % LANES * W;
-    const uint32_t low = (uint32_t)(a >> 32), high = (uint32_t)(b >> 32);  // (of keys: a and b are whole keys)
+    // (a and b are whole keys; of a row with +infinity the tokens that have it)
+    const float least = infinite ? INFINITY : logit_of((uint32_t)(a >> 32)), most = infinite ? INFINITY : logit_of((uint32_t)(b >> 32) - 1);
     for (int c0 = 0; c0 < n; c0 += U * AT_ONCE) {
       vec_t v[U];
-      int id[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int c = c0 + u * AT_ONCE + first;
-        id[u] = c < n ? m.list[c] * kChunk + in_chunk : vocab;
-        if (id[u] + W <= vocab) {
-          v[u] = *reinterpret_cast<const vec_t*>(x + id[u]);
+        const int c = c0 + u * AT_ONCE + first, id = c < n ? m.list[c] * kChunk + in_chunk : vocab;
+        if (id + W <= vocab) {
+          v[u] = *reinterpret_cast<const vec_t*>(x + id);
         } else {
 #pragma unroll
-          for (int e = 0; e < W; ++e) v[u][e] = id[u] + e < vocab ? x[id[u] + e] : (T)-INFINITY;
+          for (int e = 0; e < W; ++e) v[u][e] = id + e < vocab ? x[id + e] : (T)-INFINITY;
         }
       }
       uint32_t in = 0;
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < W; ++e) {
-          const uint32_t key = key_of(finite(logit((float)v[u][e]), infinite));
-          in |= (uint32_t)(key >= low && key < high) << (u * W + e);
-        }
+        for (int e = 0; e < W; ++e) in |= (uint32_t)((float)v[u][e] >= least && (float)v[u][e] <= most) << (u * W + e);
       const uint32_t mine = __builtin_popcount(in), upto = sums_of_wave(mine);
       uint32_t to = 0;
       if ((threadIdx.x & 63) == 63 && upto) to = atomicAdd(&m.held_count, upto);
       to = (uint32_t)__builtin_amdgcn_readlane((int)to, 63) + upto - mine;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int e = 0; e < W; ++e)
-          if (in >> (u * W + e) & 1) {
-            if (to < (uint32_t)kHeld) m.held[to] = order_of(finite(logit((float)v[u][e]), infinite), id[u] + e);
-            ++to;
-          }
+      for (; in; in &= in - 1, ++to) {
+        const int bit = __builtin_ctz(in);
+        if (to < (uint32_t)kHeld) m.held[to] = (uint32_t)(m.list[c0 + bit / W * AT_ONCE + first] * kChunk + in_chunk + bit % W);
+      }
+    }
+    __syncthreads();
+    const int held = uniform(min((int)m.held_count, kHeld));
+#pragma unroll 4
+    for (int i = threadIdx.x; i < held; i += kChoose) {
+      const int id = (int)m.held[i];
+      m.held[i] = order_of(at(id), id);
     }
   }
   __device__ __forceinline__ uint64_t fixed_at(uint64_t order) const { return fixed_of(binned(logit_of((uint32_t)(order >> 32)), r)); }

@@ -64,7 +64,7 @@ PAGED = dict(q=P, cache=P, table=P, lengths=P, ctx=P, workspace=P, ldq=1024, ldc
 @pytest.mark.parametrize("kw,words", [
     (dict(dim=80), "64, 128 or 256"), (dict(heads=9), "multiple"), (dict(kv_heads=0), "multiple"), (dict(n_requests=-1), "range"), (dict(q=None), "NULL"),
     (dict(table=None), "NULL"), (dict(workspace=None), "NULL"), (dict(workspace=P + 8), "16-byte"), (dict(ldc=1020), "16-byte"), (dict(ldq=512), "overlap"),
-    (dict(workspace_bytes=100), "too small"), (dict(n_requests=1 << 20, max_pages=1 << 20), "range")], ids=str)
+    (dict(workspace_bytes=100), "too small"), (dict(scale=float("nan")), "scale"), (dict(n_requests=1 << 20, max_pages=1 << 20), "range")], ids=str)
 def test_paged_attention_refuses(awq, lib, kw, words):
     assert refused(lib, lib.awq_paged_attention(changed(awq.AwqPagedAttentionArgs, PAGED, **kw), 3, None), words)
 
@@ -75,7 +75,7 @@ PACKED = dict(q=P, k=P, v=P, ctx=P, q_starts=P, k_starts=P, ldq=1024, ldk=256, l
 
 @pytest.mark.parametrize("kw,words", [
     (dict(dim=512), "64, 128 or 256"), (dict(heads=3), "multiple"), (dict(n_tokens=-1), "out of range"), (dict(k_starts=None, n_keys=5), "starts of their own"),
-    (dict(k=None), "NULL"), (dict(q_starts=None), "NULL"), (dict(ldv=252), "16-byte"), (dict(ctx=P + 8), "16-byte"), (dict(ldk=128), "overlap")], ids=str)
+    (dict(k=None), "NULL"), (dict(q_starts=None), "NULL"), (dict(ldv=252), "16-byte"), (dict(ctx=P + 8), "16-byte"), (dict(ldk=128), "overlap"), (dict(scale=float("inf")), "scale")], ids=str)
 def test_packed_attention_refuses(awq, lib, kw, words):
     assert refused(lib, lib.awq_packed_attention(changed(awq.AwqPackedAttentionArgs, PACKED, **kw), 1, None), words)
 

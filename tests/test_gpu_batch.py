@@ -317,7 +317,7 @@ def check_paged(got, dtype, vq, table, lengths, keys, values, spread, n_pages, s
         at, p = np.where(seen, at, 0), np.arange(L) % PAGE
         k, v, s = (x[at, :, p] for x in (keys, values, spread))
         want, size = plain.attention(vq[i:i + 1], k, v, scale, seen[None], s)
-        terms = (np.abs(vq[i]).sum(-1).max() * (np.abs(k[seen]).max() if seen.any() else 0.0)) * scale
+        terms = (np.abs(vq[i]).sum(-1).max() * (np.abs(k[seen]).max() if seen.any() else 0.0)) * abs(scale)
         limit = EPS[dtype] / 2 * np.abs(want) + (2.0 ** -11 + terms * 2.0 ** -20 + 2.0 ** -18) * size + (2.0 ** -25 if dtype == "f16" else 1e-30)
         assert (np.abs(got[i] - want[0]) <= limit[0]).all(), (i, L, np.abs(got[i] - want[0]).max(), limit.max())
 
@@ -438,7 +438,7 @@ def check_packed(got, dtype, vq, vk, vv, q_starts, k_starts, causal, scale, fill
             continue
         want, size = plain.attention(vq[a:b], vk[c:d], vv[c:d], scale, seen)
         assert (got[a:b][~seen.any(1)] == 0.0).all()
-        terms = np.abs(vq[a:b]).sum(-1).max() * np.abs(vk[c:d]).max() * scale
+        terms = np.abs(vq[a:b]).sum(-1).max() * np.abs(vk[c:d]).max() * abs(scale)
         limit = EPS[dtype] / 2 * (2 * np.abs(want) + size) * 1.01 + (terms * 2.0 ** -20 + 2.0 ** -18) * size + 1e-30
         assert (np.abs(got[a:b] - want) <= limit).all(), (a, b, nk, np.abs(got[a:b] - want).max())
     assert (got[~known] == fill).all()
@@ -506,6 +506,22 @@ def test_packed_attention_of_scores_far_from_zero(dev):
     got = packed(dev, "bf16", d_q, d_k, d_v, [0, n], None, heads, kv, dim, True, 0.125, dev.full((n, heads * dim), 9.0, "bf16")).reshape(n, heads, dim)
     assert np.isfinite(got).all()
     assert np.abs(got[0] - vv[0].reshape(kv, dim)).max() <= 2.0 ** -8 * np.abs(vv[0]).max()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_scales_that_do_not_favour_the_largest_product(dev, scale):
+    """0: all keys seen weigh the same; below 0: the least products the most"""
+    heads, kv, dim, new = 4, 2, 128, [70, 140]
+    rng = rng_of(6)
+    starts = np.cumsum([0] + new)
+    (d_q, vq), (d_k, vk), (d_v, vv) = (dev.act(rng.standard_normal((210, h * dim)), "f16") for h in (heads, kv, kv))
+    got = packed(dev, "f16", d_q, d_k, d_v, starts, None, heads, kv, dim, True, scale, dev.full((210, heads * dim), 9.0, "f16"))
+    shape = lambda x: x.reshape(210, -1, dim)  # noqa: E731
+    check_packed(shape(got), "f16", shape(vq), shape(vk), shape(vv), starts, starts, True, scale)
+    table, n_pages = tables(rng, 2, [2, 3], 4)
+    cache, k, v, spread = cache_of(dev, rng, n_pages, kv, dim)
+    got = paged(dev, "f16", d_q[:2], cache, table, [70, 140], heads, kv, dim, scale, dev.full((2, heads * dim), 9.0, "f16"))
+    check_paged(got.reshape(2, heads, dim), "f16", shape(vq)[:2], table, [70, 140], k, v, spread, n_pages, scale)
 
 
 @pytest.mark.parametrize("n", [70, 500])
