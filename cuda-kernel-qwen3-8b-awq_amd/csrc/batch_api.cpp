@@ -133,6 +133,7 @@ extern "C" int awq_packed_attention(const awq_packed_attention_args* a, int32_t 
   AWQ_REQUIRE(a->ldq >= (int64_t)a->heads * a->dim && a->ldc >= (int64_t)a->heads * a->dim && a->ldk >= (int64_t)a->kv_heads * a->dim &&
                   a->ldv >= (int64_t)a->kv_heads * a->dim,
               "rows overlap");
+  AWQ_REQUIRE(a->ldk <= 1 << 25 && a->ldv <= 1 << 25, "rows of k and v at most 2^25 values apart");
   return launch_packed_attention(*a, dtype == AWQ_DTYPE_BFLOAT16, (hipStream_t)stream);
 }
 

@@ -60,16 +60,21 @@ __device__ __forceinline__ bool find_tile(const awq_packed_attention_args& a, in
   return false;
 }
 
-// 0 in place of those that are not finite, and whether there are any
+// bits 15 and 31 of the result: some of eight 16-bit numbers are infinite or NaN
 template <typename T>
-__device__ __forceinline__ u32x4_t only_finite(u32x4_t v, bool& any) {
+__device__ __forceinline__ uint32_t not_finite(u32x4_t v) {
+  constexpr uint32_t to_bit = __is_same(T, half_t) ? 0x04000400u : 0x00800080u;
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) any |= (v[i] & 0x7fff7fffu) + to_bit;
+  return any;
+}
+// 0 in place of those that are
+template <typename T>
+__device__ __forceinline__ u32x4_t only_finite(u32x4_t v) {
   constexpr uint32_t e = __is_same(T, half_t) ? 0x7c00u : 0x7f80u;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const bool low = (v[i] & e) == e, high = (v[i] >> 16 & e) == e;
-    any |= low | high;
-    v[i] &= (low ? 0xffff0000u : 0xffffffffu) & (high ? 0x0000ffffu : 0xffffffffu);
-  }
+  for (int i = 0; i < 4; ++i) v[i] &= ((v[i] & e) == e ? 0xffff0000u : 0xffffffffu) & ((v[i] >> 16 & e) == e ? 0x0000ffffu : 0xffffffffu);
   return v;
 }
 
@@ -82,7 +87,7 @@ constexpr int kStep = 64;  // keys
 // supplies to the second product (slice j: keys 16 j + 8 (e / 4) + 4 kh + e % 4; V^T by the transposing LDS read).  Scores, maxima and sums
 // are binary32; a weight is rounded to the activations' type for the second product alone.
 // A row's 16-byte pieces lie rotated in LDS so that the rows that lanes read together are in all banks.
-// Where some query of the wavefront does not see all keys of a step, values that are not finite are kept out of the product, in which 0 times
+// Where some query of the workgroup does not see all keys of a step, values that are not finite are kept out of the product, in which 0 times
 // them is NaN, and are added for the queries that see them.
 template <typename T, int D>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_kernel(awq_packed_attention_args a) {
@@ -108,18 +113,30 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_kernel(awq_packe
   const T* const kg = (const T*)a.k + (int64_t)t.k_begin * a.ldk + (int64_t)g * D;
   const T* const vg = (const T*)a.v + (int64_t)t.k_begin * a.ldv + (int64_t)g * D;
 
-  // rotations of a row's pieces
-  const auto key_turn = [](int row) { return D == 64 ? (row >> 1) & 7 : row & 15; };
+  // rotations of a row's pieces (the same for the rows that one lane requests, 1024 / PIECES apart)
+  const auto key_turn = [](int row) { return D == 64 ? (row >> 1) & 7 : D == 128 ? row & 15 : row & 7; };
   const auto value_turn = [](int row) { return D == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1; };
+  constexpr int kApart = 256 / PIECES;
+  const int row = tid / PIECES, key_part = ((tid % PIECES) ^ key_turn(row)) * 16, value_part = ((tid % PIECES) ^ value_turn(row)) * 16;
+  const int64_t key_row = a.ldk * 2, value_row = a.ldv * 2;  // bytes
+  const uint32_t key_at = (uint32_t)row * (uint32_t)key_row + key_part, value_at = (uint32_t)row * (uint32_t)value_row + value_part;
   const auto request = [&](int k0, T* tile) __attribute__((always_inline)) {
-    const int last = end - 1 - k0;  // rows behind it are masked, and are that one again
-    const T* const kp = kg + (int64_t)k0 * a.ldk;
-    const T* const vp = vg + (int64_t)k0 * a.ldv;
+    const uint8_t* kp = (const uint8_t*)kg + k0 * key_row;
+    const uint8_t* vp = (const uint8_t*)vg + k0 * value_row;
+    T* const to = tile + wave * 512;
+    if (k0 + kStep <= end) {
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const int x = 64 * (4 * i + wave) + lane, row = x / PIECES, part = x % PIECES, from = min(row, last);
-      __builtin_amdgcn_global_load_lds((gptr_t)(kp + (int64_t)from * a.ldk + (part ^ key_turn(row)) * 8), (lptr_t)(tile + (4 * i + wave) * 512), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((gptr_t)(vp + (int64_t)from * a.ldv + (part ^ value_turn(row)) * 8), (lptr_t)(tile + kTile + (4 * i + wave) * 512), 16, 0, 0);
+      for (int i = 0; i < P; ++i, kp += kApart * key_row, vp += kApart * value_row) {
+        __builtin_amdgcn_global_load_lds((gptr_t)(kp + key_at), (lptr_t)(to + i * 2048), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((gptr_t)(vp + value_at), (lptr_t)(to + kTile + i * 2048), 16, 0, 0);
+      }
+    } else {  // rows behind the last are masked, and are that one again
+#pragma unroll 1
+      for (int i = 0; i < P; ++i) {
+        const uint32_t from = min(row + kApart * i, end - 1 - k0);
+        __builtin_amdgcn_global_load_lds((gptr_t)(kp + (from * (uint32_t)key_row + key_part)), (lptr_t)(to + i * 2048), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((gptr_t)(vp + (from * (uint32_t)value_row + value_part)), (lptr_t)(to + kTile + i * 2048), 16, 0, 0);
+      }
     }
   };
   if (end > 0) request(0, tiles);
@@ -148,10 +165,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_kernel(awq_packe
   const auto step = [&](int k0, const T* ks, auto MASKED) __attribute__((always_inline)) {
     constexpr bool masked = decltype(MASKED)::value;
     const T* const vs = ks + kTile;
-    const int L16 = lane & 15;
+    int at = lane;
+    if constexpr (D == 256) asm volatile("" : "+v"(at));  // addresses in LDS are formed anew each step: there are too many to keep
+    const int L16 = at & 15, n = at & 31, kh = at >> 5;
     // keys 16 j + 4 kh + L16 / 4 and 8 further, components 32 d + 16 ((lane / 16) % 2) + 4 (L16 % 4) .. + 3
     const auto values = [&](int j, int d) __attribute__((always_inline)) {
-      const int row = 16 * j + 4 * kh + (L16 >> 2), piece = 4 * d + 2 * ((lane >> 4) & 1) + ((L16 >> 1) & 1);
+      const int row = 16 * j + 4 * kh + (L16 >> 2), piece = 4 * d + 2 * ((at >> 4) & 1) + ((L16 >> 1) & 1);
       const T* const lp = vs + row * D + (piece ^ value_turn(row)) * 8 + (L16 & 1) * 4;
       const T* const up = vs + (row + 8) * D + (piece ^ value_turn(row + 8)) * 8 + (L16 & 1) * 4;
       const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4_t __attribute__((address_space(3)))*)lp);
@@ -165,18 +184,21 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_kernel(awq_packe
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[half][i] = 0.0f;
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d)
+    for (int d = 0; d < D / 16; ++d) {
+      if (D == 256 && d % 4 == 0) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int row = 32 * half + n;
         s[half] = product(*reinterpret_cast<const eight_t*>(ks + row * D + ((2 * d + kh) ^ key_turn(row)) * 8), qop[d], s[half]);
       }
+    }
     // s[half][i]: key k0 + 32 half + 8 (i / 4) + 4 kh + i % 4
     if constexpr (masked) {
+      const int sees = seen - k0 - 4 * kh;
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[half][i] = k0 + 32 * half + 8 * (i >> 2) + 4 * kh + (i & 3) < seen ? s[half][i] : -INFINITY;
+        for (int i = 0; i < 16; ++i) s[half][i] = 32 * half + 8 * (i >> 2) + (i & 3) < sees ? s[half][i] : -INFINITY;
     }
     float mx = s[0][0];
 #pragma unroll
@@ -206,38 +228,50 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_kernel(awq_packe
         l_run += p;
         pop[2 * half + (i >> 3)][i & 7] = (T)p;
       }
-    bool strange = false;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int d = 0; d < D / 32; ++d) {
-        eight_t v = values(j, d);
-        if constexpr (masked) v = __builtin_bit_cast(eight_t, only_finite<T>(__builtin_bit_cast(u32x4_t, v), strange));
-        o[d] = product(v, pop[j], o[d]);
+        if (D == 256 && d % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+        o[d] = product(values(j, d), pop[j], o[d]);
       }
-    if constexpr (masked) {
-      if (__builtin_amdgcn_ballot_w64(strange)) {
-#pragma unroll 1
-        for (int key = k0; key < min(k0 + kStep, most); ++key) {
-          const T* const v = vg + (int64_t)key * a.ldv + 4 * kh;
-#pragma unroll
-          for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              const float x = (float)v[32 * d + 8 * (c >> 2) + (c & 3)];
-              if (key < seen && !(fabsf(x) < INFINITY)) o[d][c] += x;
-            }
-        }
-      }
-    }
   };
+  const int unmasked = seen_by(min(t.first, nq - 1));  // keys that all queries of the workgroup see
   T* ks = tiles;
   for (int k0 = 0; k0 < end; k0 += kStep) {
     __syncthreads();  // these keys and values are there, the last ones' readers done
+    bool strange = false;
+    if (k0 + kStep > unmasked) {
+      u32x4_t* const vs = reinterpret_cast<u32x4_t*>(ks + kTile) + tid;
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < P; ++i) any |= not_finite<T>(vs[256 * i]);
+      strange = __syncthreads_or(any & 0x80008000u) != 0;
+      if (strange) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) vs[256 * i] = only_finite<T>(vs[256 * i]);
+        __syncthreads();
+      }
+    }
     T* const other = tiles + (ks == tiles ? 2 * kTile : 0);
     if (k0 + kStep < end) request(k0 + kStep, other);
     if (k0 + kStep <= least) step(k0, ks, std::false_type());
     else if (k0 < most) step(k0, ks, std::true_type());
+    if (strange) {
+#pragma unroll 1
+      for (int key = k0; key < min(k0 + kStep, most); ++key) {
+        const T* const v = vg + (int64_t)key * a.ldv + 4 * kh;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) {
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const float x = (float)v[32 * d + 8 * (c >> 2) + (c & 3)];
+            o[d][c] += key < seen && !(fabsf(x) < INFINITY) ? x : 0.0f;
+          }
+        }
+      }
+    }
     ks = other;
   }
   if (qi >= nq) return;

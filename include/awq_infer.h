@@ -825,7 +825,7 @@ int awq_paged_attention(const awq_paged_attention_args* args, int32_t dtype, voi
  * q_starts[i] .. q_starts[i + 1] - 1 and the keys k_starts[i] .. k_starts[i + 1] - 1 (k_starts NULL: as
  * q_starts), both ascending, on the device.  causal != 0: the last query sees all keys and
  * each query ahead of it one fewer; 0: all see all.  A query without keys: zeros.  Rows of ctx that belong to no request stay as they
- * were.  n_tokens, n_keys: rows of q and of k and v. */
+ * were.  n_tokens, n_keys: rows of q and of k and v; those of k and v are at most 2^25 values apart. */
 typedef struct awq_packed_attention_args {
   const void* q;
   const void* k;

@@ -75,7 +75,8 @@ PACKED = dict(q=P, k=P, v=P, ctx=P, q_starts=P, k_starts=P, ldq=1024, ldk=256, l
 
 @pytest.mark.parametrize("kw,words", [
     (dict(dim=512), "64, 128 or 256"), (dict(heads=3), "multiple"), (dict(n_tokens=-1), "out of range"), (dict(k_starts=None, n_keys=5), "starts of their own"),
-    (dict(k=None), "NULL"), (dict(q_starts=None), "NULL"), (dict(ldv=252), "16-byte"), (dict(ctx=P + 8), "16-byte"), (dict(ldk=128), "overlap"), (dict(scale=float("inf")), "scale")], ids=str)
+    (dict(k=None), "NULL"), (dict(q_starts=None), "NULL"), (dict(ldv=252), "16-byte"), (dict(ctx=P + 8), "16-byte"), (dict(ldk=128), "overlap"), (dict(scale=float("inf")), "scale"),
+    (dict(ldv=(1 << 25) + 8), "apart")], ids=str)
 def test_packed_attention_refuses(awq, lib, kw, words):
     assert refused(lib, lib.awq_packed_attention(changed(awq.AwqPackedAttentionArgs, PACKED, **kw), 1, None), words)
 
