@@ -78,8 +78,6 @@ __device__ __forceinline__ u32x4_t only_finite(u32x4_t v) {
   return v;
 }
 
-constexpr int kStep = 64;  // keys
-
 // 128 queries of one head a workgroup, 32 a wavefront; 64 keys and values at a time come into LDS by themselves, the next ones while these are
 // multiplied.  Queries are columns throughout, lane (n, kh) = (lane % 32, lane / 32):
 //     S^T[key][query] = K Q^T,   O^T[c][query] += V^T P^T      v_mfma_f32_32x32x16
@@ -89,13 +87,13 @@ constexpr int kStep = 64;  // keys
 // A row's 16-byte pieces lie rotated in LDS so that the rows that lanes read together are in all banks.
 // Where some query of the workgroup does not see all keys of a step, values that are not finite are kept out of the product, in which 0 times
 // them is NaN, and are added for the queries that see them.
-template <typename T, int D>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_kernel(awq_packed_attention_args a) {
+template <typename T, int D, int kStep, int WAVES>
+__global__ __launch_bounds__(256, WAVES) void packed_kernel(awq_packed_attention_args a) {
   typedef typename Vec<T>::eight eight_t;
   typedef typename Vec<T>::four four_t;
   typedef __attribute__((address_space(1))) const void* gptr_t;
   typedef __attribute__((address_space(3))) void* lptr_t;
-  constexpr int PIECES = D / 8, P = D / 32;  // of a row; requests of a wavefront for 64 keys
+  constexpr int PIECES = D / 8, P = kStep * D / 2048;  // of a row; requests of a wavefront for a step's keys
   constexpr int kTile = kStep * D;
   __shared__ __attribute__((aligned(16))) T tiles[4 * kTile];  // keys, values, keys, values
   const int group = a.heads / a.kv_heads;
@@ -162,8 +160,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_kernel(awq_packe
   float m_run = -INFINITY, l_run = 0.0f;  // (of this lane's keys alone)
   const float mul = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 0x1p-126f);  // (0 times -infinity would be NaN)
 
-  const auto step = [&](int k0, const T* ks, auto MASKED) __attribute__((always_inline)) {
-    constexpr bool masked = decltype(MASKED)::value;
+  const auto step = [&](int k0, const T* ks) __attribute__((always_inline)) {
     const T* const vs = ks + kTile;
     int at = lane;
     if constexpr (D == 256) asm volatile("" : "+v"(at));  // addresses in LDS are formed anew each step: there are too many to keep
@@ -178,31 +175,31 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_kernel(awq_packe
       const four_t l4 = __builtin_bit_cast(four_t, lo), u4 = __builtin_bit_cast(four_t, hi);
       return eight_t{l4[0], l4[1], l4[2], l4[3], u4[0], u4[1], u4[2], u4[3]};
     };
-    f32x16_t s[2];
+    f32x16_t s[kStep / 32];
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
+    for (int half = 0; half < kStep / 32; ++half)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[half][i] = 0.0f;
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) {
       if (D == 256 && d % 4 == 0) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int half = 0; half < kStep / 32; ++half) {
         const int row = 32 * half + n;
         s[half] = product(*reinterpret_cast<const eight_t*>(ks + row * D + ((2 * d + kh) ^ key_turn(row)) * 8), qop[d], s[half]);
       }
     }
     // s[half][i]: key k0 + 32 half + 8 (i / 4) + 4 kh + i % 4
-    if constexpr (masked) {
+    if (k0 + kStep > least) {
       const int sees = seen - k0 - 4 * kh;
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
+      for (int half = 0; half < kStep / 32; ++half)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[half][i] = 32 * half + 8 * (i >> 2) + (i & 3) < sees ? s[half][i] : -INFINITY;
     }
     float mx = s[0][0];
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
+    for (int half = 0; half < kStep / 32; ++half)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[half][i]);
     const HalfPair best = half_pair(mx);
@@ -213,15 +210,15 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_kernel(awq_packe
       scale = 1.0f;
       mx *= mul;
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
+      for (int half = 0; half < kStep / 32; ++half)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[half][i] *= mul;
     }
     move_maximum<true>(mx > -INFINITY ? mx * scale : -INFINITY, m_run, l_run, o);
     const float from = m_run == -INFINITY ? 0.0f : m_run;  // (no key seen yet: all weights are 0)
-    eight_t pop[4];
+    eight_t pop[kStep / 16];
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
+    for (int half = 0; half < kStep / 32; ++half)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[half][i], scale, -from));
@@ -229,7 +226,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_kernel(awq_packe
         pop[2 * half + (i >> 3)][i & 7] = (T)p;
       }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < kStep / 16; ++j)
 #pragma unroll
       for (int d = 0; d < D / 32; ++d) {
         if (D == 256 && d % 4 == 0) __builtin_amdgcn_sched_barrier(0);
@@ -255,8 +252,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_kernel(awq_packe
     }
     T* const other = tiles + (ks == tiles ? 2 * kTile : 0);
     if (k0 + kStep < end) request(k0 + kStep, other);
-    if (k0 + kStep <= least) step(k0, ks, std::false_type());
-    else if (k0 < most) step(k0, ks, std::true_type());
+    if (k0 < most) step(k0, ks);
     if (strange) {
 #pragma unroll 1
       for (int key = k0; key < min(k0 + kStep, most); ++key) {
@@ -294,9 +290,9 @@ int launch(const awq_packed_attention_args& a, hipStream_t st) {
   const int64_t tiles = a.n_tokens / kQueries + std::min<int64_t>(a.n_requests, a.n_tokens);
   AWQ_REQUIRE(tiles * a.heads < (1ll << 31), "too many queries and heads");
   const dim3 grid((unsigned)(tiles * a.heads));
-  if (a.dim == 64) hipLaunchKernelGGL((packed_kernel<T, 64>), grid, dim3(256), 0, st, a);
-  else if (a.dim == 128) hipLaunchKernelGGL((packed_kernel<T, 128>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((packed_kernel<T, 256>), grid, dim3(256), 0, st, a);
+  if (a.dim == 64) hipLaunchKernelGGL((packed_kernel<T, 64, 64, 3>), grid, dim3(256), 0, st, a);
+  else if (a.dim == 128) hipLaunchKernelGGL((packed_kernel<T, 128, 64, 2>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((packed_kernel<T, 256, 64, 1>), grid, dim3(256), 0, st, a);
   AWQ_HIP_TRY(hipGetLastError());
   return AWQ_OK;
 }
