@@ -76,4 +76,28 @@ __device__ __forceinline__ float sum_apart(float v, int n) {
   return a + b;
 }
 
+// in every lane the sum over the lanes up to it, itself included (4 or 8 bytes): within rows of 16, then the rows ahead
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T ahead(T v) {  // 0 where there is none
+  static_assert(sizeof(T) == 4 || sizeof(T) == 8, "one or two registers");
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+  } else {
+    const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+    const unsigned int lo = (unsigned int)__builtin_amdgcn_update_dpp(0, (int)(unsigned int)u, CTRL, ROWS, 0xf, false);
+    const unsigned int hi = (unsigned int)__builtin_amdgcn_update_dpp(0, (int)(unsigned int)(u >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(T, (unsigned long long)hi << 32 | lo);
+  }
+}
+template <typename T>
+__device__ __forceinline__ T upto(T v) {
+  v += ahead<0x111, 0xf>(v);
+  v += ahead<0x112, 0xf>(v);
+  v += ahead<0x114, 0xf>(v);
+  v += ahead<0x118, 0xf>(v);
+  v += ahead<0x142, 0xa>(v);  // lane 15 of the row ahead, for rows 1 and 3
+  v += ahead<0x143, 0xc>(v);  // lane 31, for rows 2 and 3
+  return v;
+}
+
 }  // namespace lanes

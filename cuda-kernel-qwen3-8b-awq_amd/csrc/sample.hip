@@ -12,7 +12,7 @@ namespace {
 //   scan_kernel    parts of 8,192 logits: largest, sum of weights, and where a row is filtered a histogram, sums and counts by bin
 //   choose_kernel  a workgroup a row: the bin in which the tokens kept end, the order within that bin alone, the part that the uniform
 //                  number falls in, and the token in that part.
-constexpr int kPart = 8192, kScan = 256, kChoose = 512, kBins = 512, kDigits = 256, kChunk = 32, kHeld = 8192, kFew = 512, kMostParts = 64;
+constexpr int kPart = 8192, kScan = 256, kChoose = 512, kBins = 512, kDigits = 256, kChunk = 32, kHeld = 8192, kFew = 128, kMostParts = 64;
 constexpr int kMostChunks = kMostParts * kPart / kChunk, kCopies = 8;
 constexpr int kFixed = 36, kCountShift = 50;
 constexpr uint64_t kSumMask = (1ull << kCountShift) - 1;
@@ -38,6 +38,12 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 __device__ __forceinline__ float uniform(float v) { return __uint_as_float(uniform(__float_as_uint(v))); }
 __device__ __forceinline__ uint64_t uniform(uint64_t v) { return (uint64_t)uniform((uint32_t)(v >> 32)) << 32 | uniform((uint32_t)v); }
 __device__ __forceinline__ double uniform(double v) { return __longlong_as_double((long long)uniform((uint64_t)__double_as_longlong(v))); }
+
+__device__ __forceinline__ double last_lane(double v) {
+  const uint64_t u = (uint64_t)__double_as_longlong(v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, 63), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 63);
+  return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
 
 struct Row {
   double per_t;  // 8 / T
@@ -232,17 +238,6 @@ struct ChooseMemory {
   int pick, last;
 };
 
-template <typename T>
-__device__ __forceinline__ T sums_of_wave(T v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const T u = __shfl_up(v, off, 64);
-    if (lane >= off) v += u;
-  }
-  return v;
-}
-
 // The first of 64 N entries, N a lane, at which `full` holds of the sums up to it (itself included), and the sums ahead of it; 64 N: none.
 // Every wavefront finds it for itself.
 template <typename S>
@@ -258,9 +253,8 @@ __device__ __forceinline__ Found<S> first_full(const S (&sum)[N], const uint32_t
   uint32_t many = count[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) mine += sum[i], many += count[i];
-  const S up = __shfl_up(sums_of_wave(mine), 1, 64);  // (the sums ahead as they are formed, not as a difference)
-  S s = lane ? up : (S)0;
-  uint32_t n = sums_of_wave(many) - many;
+  S s = lanes::ahead<0x138, 0xf>(lanes::upto(mine));  // the sums ahead as they are formed, not as a difference
+  uint32_t n = lanes::upto(many) - many;
   int at = N;
   S before = s;
   uint32_t before_count = n;
@@ -290,28 +284,34 @@ struct Choose {
   double top;     // its bin
   bool infinite;
 
-  __device__ __forceinline__ float at(int i) const { return finite(logit((float)x[i]), infinite); }
+  __device__ __forceinline__ float of(T v) const { return finite(logit((float)v), infinite); }
+  __device__ __forceinline__ float at(int i) const { return of(x[i]); }
   // distance of a logit's bin from the row's first; kBins: further or no weight
   __device__ __forceinline__ int below(const Binned& b, float l) const {
     const double d = top - b.bin;
     return l == -INFINITY || !(d < kBins) ? kBins : (int)d;
   }
-  // the lowest order of a logit in bin j or ahead of it, by 64 guesses at a time
+  // the lowest order of a logit in bin j or ahead of it: among the 64 around the quotient, or else by 64 guesses at a time
   __device__ __forceinline__ uint32_t lowest_key(int j) const {
+    const uint32_t lane = threadIdx.x & 63;
     uint32_t lo = key_of(-INFINITY), hi = uniform(key_of(largest));  // not in it, in it
+    const auto in_bin = [&](uint32_t guess) __attribute__((always_inline)) { return guess >= hi || (guess > lo && top - bin_of(logit_of(guess), r) <= j); };
+    const uint32_t around = uniform(key_of((float)((top - j) / r.per_t))) - 31;
+    const unsigned long long near = __builtin_amdgcn_ballot_w64(in_bin(around + lane));
+    if (near != 0 && !(near & 1)) return around + (uint32_t)__builtin_ctzll(near);
     for (int turn = 0; turn < 6 && hi - lo > 1; ++turn) {  // (2^32 in six turns)
-      const uint32_t step = (hi - lo + 63) / 64, guess = lo + step * ((threadIdx.x & 63) + 1);
-      const bool in = guess >= hi || top - bin_of(logit_of(guess), r) <= j;
-      const uint32_t first = __builtin_ctzll(__builtin_amdgcn_ballot_w64(in) | 1ull << 63);  // (the last lane's guess is not below hi)
+      const uint32_t step = (hi - lo + 63) / 64;
+      const unsigned long long in = __builtin_amdgcn_ballot_w64(in_bin(lo + step * (lane + 1)));
+      const uint32_t first = __builtin_ctzll(in | 1ull << 63);  // (the last lane's guess is not below hi)
       hi = min(hi, lo + step * (first + 1));
       lo = lo + step * first;
     }
     return hi;
   }
-  // the tokens of the orders a .. b - 1 into `held`, out of the row, by the chunks listed: 16 bytes of a chunk a thread and four of them at once.
+  // the tokens of the orders a .. b - 1 into `held`, out of the row, by the chunks listed: 16 bytes of a chunk a thread and 64 logits at once.
   // First their ids, which a few lanes have at a time; then a logit a thread.
   __device__ __forceinline__ void hold(uint64_t a, uint64_t b) const {
-    constexpr int W = 16 / sizeof(T), LANES = kChunk / W, AT_ONCE = kChoose / LANES, U = 4;
+    constexpr int W = 16 / sizeof(T), LANES = kChunk / W, AT_ONCE = kChoose / LANES, U = 64 / W;
     typedef typename Some<T, W>::type vec_t;
     const int vocab = (int)s.a.vocab, n = uniform((int)m.list_count), first = threadIdx.x / LANES, in_chunk = threadIdx.x % LANES * W;
     // (a and b are whole keys; of a row with +infinity the tokens that have it)
@@ -320,6 +320,7 @@ struct Choose {
       vec_t v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
+        if (c0 + u * AT_ONCE >= n) break;
         const int c = c0 + u * AT_ONCE + first, id = c < n ? m.list[c] * kChunk + in_chunk : vocab;
         if (id + W <= vocab) {
           v[u] = *reinterpret_cast<const vec_t*>(x + id);
@@ -328,17 +329,19 @@ struct Choose {
           for (int e = 0; e < W; ++e) v[u][e] = id + e < vocab ? x[id + e] : (T)-INFINITY;
         }
       }
-      uint32_t in = 0;
+      uint64_t in = 0;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        if (c0 + u * AT_ONCE >= n) break;
 #pragma unroll
-        for (int e = 0; e < W; ++e) in |= (uint32_t)((float)v[u][e] >= least && (float)v[u][e] <= most) << (u * W + e);
-      const uint32_t mine = __builtin_popcount(in), upto = sums_of_wave(mine);
+        for (int e = 0; e < W; ++e) in |= (uint64_t)((float)v[u][e] >= least && (float)v[u][e] <= most) << (u * W + e);
+      }
+      const uint32_t mine = __builtin_popcountll(in), upto = lanes::upto(mine);
       uint32_t to = 0;
       if ((threadIdx.x & 63) == 63 && upto) to = atomicAdd(&m.held_count, upto);
       to = (uint32_t)__builtin_amdgcn_readlane((int)to, 63) + upto - mine;
       for (; in; in &= in - 1, ++to) {
-        const int bit = __builtin_ctz(in);
+        const int bit = __builtin_ctzll(in);
         if (to < (uint32_t)kHeld) m.held[to] = (uint32_t)(m.list[c0 + bit / W * AT_ONCE + first] * kChunk + in_chunk + bit % W);
       }
     }
@@ -376,7 +379,7 @@ struct Choose {
     if (threadIdx.x == 0) m.held_count = m.list_count = 0;
     __syncthreads();
     const int lane = threadIdx.x & 63;
-    constexpr int U = 4;
+    constexpr int U = 10;
     for (int c0 = 0; c0 < s.chunks; c0 += U * kChoose) {
       float largest_of[U];
 #pragma unroll
@@ -384,16 +387,16 @@ struct Choose {
         const int c = c0 + u * kChoose + threadIdx.x;
         largest_of[u] = c < s.chunks ? chunk[c] : -INFINITY;
       }
+      uint32_t mine = 0;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const bool some = key_of(finite(largest_of[u], infinite)) >= low;
-        const unsigned long long any = __builtin_amdgcn_ballot_w64(some);
-        if (any == 0) continue;
-        uint32_t to = 0;
-        if (lane == 0) to = atomicAdd(&m.list_count, (uint32_t)__builtin_popcountll(any));
-        to = uniform(to) + __builtin_popcountll(any & ((1ull << lane) - 1));
-        if (some) m.list[to] = (uint16_t)(c0 + u * kChoose + threadIdx.x);
-      }
+      for (int u = 0; u < U; ++u) mine += key_of(finite(largest_of[u], infinite)) >= low;
+      const uint32_t upto = lanes::upto(mine);
+      uint32_t to = 0;
+      if (lane == 63 && upto) to = atomicAdd(&m.list_count, upto);
+      to = (uint32_t)__builtin_amdgcn_readlane((int)to, 63) + upto - mine;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (key_of(finite(largest_of[u], infinite)) >= low) m.list[to++] = (uint16_t)(c0 + u * kChoose + threadIdx.x);
     }
     __syncthreads();
     if (n > kHeld) return;
@@ -453,8 +456,13 @@ struct Choose {
     const uint64_t order = mine < n ? m.few[mine] : ~0ull;
     uint64_t sum = 0;
     uint32_t count = 0;
-    for (int i = tid % wide; i < n; i += wide)
-      if (m.few[i] > order) ++count, sum += m.few_weight[i];
+#pragma unroll 4
+    for (int i = tid % wide; i < n; i += wide) {
+      const uint64_t weight = m.few_weight[i];
+      const bool before = m.few[i] > order;
+      count += before;
+      sum += before ? weight : 0;
+    }
     for (int off = wide / 2; off > 0; off >>= 1) {
       sum += __shfl_xor(sum, off, 64);
       count += __shfl_xor(count, off, 64);
@@ -476,18 +484,15 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
   const int64_t row = blockIdx.x;
   if (tid < S) m.part[tid] = s.part[row * S + tid];
   const Row r = row_of(a, row);
-  static_assert(kBins <= kChoose, "a thread a bin");
-  if (!r.greedy && tid < kBins) {
+  static_assert(kBins == kChoose, "a thread a bin");
+  if (!r.greedy) {
     m.table[tid] = exp(-0.125 * tid);
-    m.fixed[tid] = 0;
-    m.bin_count[tid] = 0;
   }
   if (tid < kMostParts) m.in_bin[tid] = 0;
   if (tid == 0) m.pick = INT32_MAX, m.last = 0;
+  const float uniform_number = a.uniform[row];
   __syncthreads();
-  float largest = -INFINITY;
-  for (int i = 0; i < S; ++i) largest = fmaxf(largest, m.part[i].largest);
-  largest = uniform(largest);
+  float largest = uniform(lanes::maximum<64>(lane < S ? m.part[lane].largest : -INFINITY));
   if (r.greedy || largest == -INFINITY) {
     if (tid == 0) {
       int id = 0;
@@ -520,13 +525,22 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
   const double heaviest = uniform((double)largest * r.per_t * 0.125);
   const auto heavy = [&](float l) { return exp((double)l * r.per_t * 0.125 - heaviest) >= (double)r.min_p; };
   if (r.filtered) {
-    for (int i = tid / kBins; i < S; i += kChoose / kBins) {
-      const int j = m.behind[i] + tid % kBins;
-      if (j >= kBins) continue;
-      const uint64_t h = histogram[i * kBins + tid % kBins];
-      if (h == 0) continue;
-      atomicAdd((unsigned long long*)&m.fixed[j], (unsigned long long)(h & kSumMask));
-      atomicAdd(&m.bin_count[j], (uint32_t)(h >> kCountShift));
+    {  // a bin of the row a thread
+      uint64_t fixed = 0;
+      uint32_t count = 0;
+      constexpr int U = 20;
+      for (int i0 = 0; i0 < S; i0 += U) {
+        uint64_t h[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int i = min(i0 + u, S - 1), b = tid - m.behind[i];
+          h[u] = i0 + u < S && b >= 0 ? histogram[i * kBins + b] : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) fixed += h[u] & kSumMask, count += (uint32_t)(h[u] >> kCountShift);
+      }
+      m.fixed[tid] = fixed;
+      m.bin_count[tid] = count;
     }
     __syncthreads();
     constexpr int N = kBins / 64;
@@ -538,9 +552,7 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
       count[i] = m.bin_count[N * lane + i];
       all += sum[i];
     }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) all += __shfl_xor(all, off, 64);
-    all = uniform(all);
+    all = last_lane(lanes::upto(all));
     uint64_t from = 0, to = 0;  // the orders of bin `end`
     // top-k, top-p and min-p, each within what those ahead of it keep
 #pragma unroll 1
@@ -588,34 +600,46 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
           atomicAdd((unsigned long long*)&m.in_bin[(uint32_t)~(uint32_t)order / kPart], (unsigned long long)c.fixed_at(order));
       });
     __syncthreads();
-    for (int i = wave; i < S; i += kChoose / 64) {
-      double part = 0.0;
-      for (int b = lane; b + m.behind[i] < end; b += 64) part += (double)(histogram[i * kBins + b] & kSumMask) * kUnit * m.table[b + m.behind[i]];
+    constexpr int U = 4, WAVES = kChoose / 64;
+    for (int i0 = wave; i0 < S; i0 += U * WAVES) {
+      uint64_t h[U][2];  // of four parts the first 128 bins: mostly that is all
 #pragma unroll
-      for (int off = 32; off > 0; off >>= 1) part += __shfl_xor(part, off, 64);
-      if (lane == 0) m.part_sum[i] = end < kBins ? part + (double)m.in_bin[i] * kUnit * m.table[end] : part;
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const int i = i0 + u * WAVES, b = 64 * v + lane;
+          h[u][v] = i < S && b + m.behind[i] < end ? histogram[i * kBins + b] : 0;
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * WAVES;
+        if (i >= S) break;
+        const int behind = m.behind[i];
+        double part = 0.0;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) part += (double)(h[u][v] & kSumMask) * kUnit * m.table[min(64 * v + lane + behind, kBins - 1)];
+        for (int b = 128 + lane; b + behind < end; b += 64) part += (double)(histogram[i * kBins + b] & kSumMask) * kUnit * m.table[b + behind];
+        part = lanes::upto(part);
+        if (lane == 63) m.part_sum[i] = end < kBins ? part + (double)m.in_bin[i] * kUnit * m.table[end] : part;
+      }
     }
   } else if (tid < S) {
     m.part_sum[tid] = m.behind[tid] < kBins ? m.part[tid].sum * m.table[m.behind[tid]] : 0.0;
   }
   __syncthreads();
-  double total = 0.0;
-  for (int i = 0; i < S; ++i) total += m.part_sum[i];
-  const double target = (double)fminf(fmaxf(a.uniform[row], 0.0f), 0x1.fffffep-1f) * total;
-  double base = 0.0;
-  int part = -1;  // (a row has some weight, and so has one of its parts)
-  for (int i = 0; i < S; ++i) {
-    if (m.part_sum[i] <= 0.0) continue;
-    if (part >= 0) base += m.part_sum[part];
-    part = i;
-    if (base + m.part_sum[i] > target) break;
-  }
-  part = max(part, 0);
+  const double of_part[1] = {lane < S ? m.part_sum[lane] : 0.0};
+  const double total = last_lane(lanes::upto(of_part[0]));
+  const double target = (double)fminf(fmaxf(uniform_number, 0.0f), 0x1.fffffep-1f) * total;
+  const uint32_t nothing[1] = {0};
+  static_assert(kMostParts == 64, "a part a lane");
+  const Found<double> in_part = first_full(of_part, nothing, [&](double su, uint32_t) { return su > target; });
+  double base = in_part.sum;
+  int part = in_part.at < 64 ? in_part.at : 0;  // (a row has some weight, so one of its parts is it)
   // A uniform number this close to 0 asks for the first tokens, whose weights may be those that the sums do without: part after part.
   const bool least = target < total * 0x1p-60;
   if (least) base = 0.0, part = 0;
-  const auto weight_at = [&](int id) __attribute__((always_inline)) {
-    const float l = c.at(id);
+  const auto weight_of_token = [&](T logit_of_it, int id) __attribute__((always_inline)) {
+    const float l = c.of(logit_of_it);
     const Binned b = binned(l, r);
     const int j = c.below(b, l);
     if (j < end || (j == end && j < kBins && order_of(l, id) >= border && (!at_least || heavy(l)))) return weight_of(b) * m.table[j];
@@ -626,9 +650,23 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
     // sixteen logits of the part a thread, in order; then those of the thread that the number falls in, one a lane
     double sum = 0.0;
     const int at = part * kPart + tid * kEach;
-#pragma unroll 4
-    for (int e = 0; e < kEach; ++e) sum += at + e < a.vocab ? weight_at(at + e) : 0.0;
-    double before = sums_of_wave(sum);
+    typedef typename Some<T, 16 / sizeof(T)>::type vec_t;
+    constexpr int W = 16 / sizeof(T), L = kEach / W;
+    vec_t v[L];
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      if (at + (i + 1) * W <= a.vocab) {
+        v[i] = *reinterpret_cast<const vec_t*>(c.x + at + i * W);
+      } else {
+#pragma unroll
+        for (int e = 0; e < W; ++e) v[i][e] = at + i * W + e < a.vocab ? c.x[at + i * W + e] : (T)-INFINITY;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+#pragma unroll
+      for (int e = 0; e < W; ++e) sum += weight_of_token(v[i][e], at + i * W + e);
+    double before = lanes::upto(sum);
     if (lane == 63) m.wave_sum[wave] = before;
     __syncthreads();
     before += base;
@@ -637,10 +675,9 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
       if (w < wave) before += m.wave_sum[w];
       base += m.wave_sum[w];
     }
-    if (sum > 0.0) {
-      atomicMax(&m.last, tid);  // (of the last part that is looked at)
-      if (before > target) atomicMin(&m.pick, tid);
-    }
+    const unsigned long long some = __builtin_amdgcn_ballot_w64(sum > 0.0), over = __builtin_amdgcn_ballot_w64(sum > 0.0 && before > target);
+    if (lane == 0 && some) atomicMax(&m.last, tid + 63 - __builtin_clzll(some));  // (of the last part that is looked at)
+    if (lane == 0 && over) atomicMin(&m.pick, tid + __builtin_ctzll(over));
     if (tid < kChoose) m.until[tid] = before - sum;
     __syncthreads();
     if (!least || m.pick != INT32_MAX || part + 1 == S) break;
@@ -648,8 +685,8 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
   }
   if (wave == 0) {
     const int thread = m.pick == INT32_MAX ? m.last : m.pick, id = part * kPart + thread * kEach + lane;
-    const double w = lane < kEach && id < a.vocab ? weight_at(id) : 0.0;
-    const double before = m.until[thread] + sums_of_wave(w);
+    const double w = lane < kEach && id < a.vocab ? weight_of_token(c.x[id], id) : 0.0;
+    const double before = m.until[thread] + lanes::upto(w);
     const unsigned long long over = __builtin_amdgcn_ballot_w64(w > 0.0 && before > target), some = __builtin_amdgcn_ballot_w64(w > 0.0);
     // (a rounding away from the end: the last one kept)
     const int of_thread = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : 0;
