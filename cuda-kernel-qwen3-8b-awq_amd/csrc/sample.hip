@@ -232,6 +232,7 @@ struct ChooseMemory {
   uint64_t fixed[kBins];
   uint32_t bin_count[kBins];
   double table[kBins], part_sum[kMostParts], wave_sum[kChoose / 64], until[kChoose];
+  uint32_t wave_count[kChoose / 64];
   Part part[kMostParts];
   int behind[kMostParts];
   uint32_t held_count, list_count, few_count;
@@ -521,6 +522,7 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
 
   int end = kBins;          // bins below it are kept whole, those above it not at all
   uint64_t border = 0;      // of bin `end` the tokens that are not behind this in order
+  float lightest = -INFINITY;  // no token behind this logit is kept
   bool at_least = false;    // and those of them that weigh at least min_p
   const double heaviest = uniform((double)largest * r.per_t * 0.125);
   const auto heavy = [&](float l) { return exp((double)l * r.per_t * 0.125 - heaviest) >= (double)r.min_p; };
@@ -541,18 +543,30 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
       }
       m.fixed[tid] = fixed;
       m.bin_count[tid] = count;
+      const double of_wave = lanes::upto((double)fixed * kUnit * m.table[tid]);
+      count = lanes::upto(count);
+      if (lane == 63) m.wave_sum[wave] = of_wave, m.wave_count[wave] = count;
     }
     __syncthreads();
+    // the first bin at which `full` holds of the sums up to it: of 64 bins together, then of theirs; every wavefront for itself
     constexpr int N = kBins / 64;
-    double sum[N], all = 0.0;
-    uint32_t count[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      sum[i] = (double)m.fixed[N * lane + i] * kUnit * m.table[N * lane + i];
-      count[i] = m.bin_count[N * lane + i];
-      all += sum[i];
-    }
-    all = last_lane(lanes::upto(all));
+    const double of_many = lane < N ? m.wave_sum[lane] : 0.0;
+    const uint32_t count_of_many = lane < N ? m.wave_count[lane] : 0;
+    const double many_upto = lanes::upto(of_many), many_ahead = lanes::ahead<0x138, 0xf>(many_upto);
+    const uint32_t count_ahead = lanes::upto(count_of_many) - count_of_many;
+    const auto first_bin = [&](auto full) __attribute__((always_inline)) {
+      const unsigned long long any = __builtin_amdgcn_ballot_w64(lane < N && full(many_ahead + of_many, count_ahead + count_of_many));
+      if (any == 0) return Found<double>{kBins, 0.0, 0};
+      const int many = __builtin_ctzll(any), bin = 64 * many + lane;
+      const double base = uniform(__shfl(many_ahead, many, 64));
+      const uint32_t base_count = uniform((uint32_t)__shfl((int)count_ahead, many, 64)), count = m.bin_count[bin];
+      const double upto = lanes::upto((double)m.fixed[bin] * kUnit * m.table[bin]), ahead = base + lanes::ahead<0x138, 0xf>(upto);
+      const uint32_t count_upto = lanes::upto(count);
+      // (the last of them has the sums that were looked at)
+      const int from = __builtin_ctzll(__builtin_amdgcn_ballot_w64(full(base + upto, base_count + count_upto)) | 1ull << 63);
+      return Found<double>{64 * many + from, uniform(__shfl(ahead, from, 64)), base_count + uniform((uint32_t)__shfl((int)(count_upto - count), from, 64))};
+    };
+    double all = last_lane(many_upto);
     uint64_t from = 0, to = 0;  // the orders of bin `end`
     // top-k, top-p and min-p, each within what those ahead of it keep
 #pragma unroll 1
@@ -563,7 +577,7 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
       if (filter < 2) {
         if (filter == 0 ? r.top_k == 0 : !(r.top_p < 1.0f)) continue;
         const double target = (double)r.top_p * all;
-        Found<double> f = first_full(sum, count, [&](double su, uint32_t n) { return filter ? su >= target : n >= (uint32_t)r.top_k; });
+        Found<double> f = first_bin([&](double su, uint32_t n) { return filter ? su >= target : n >= (uint32_t)r.top_k; });
         if (f.at == kBins) continue;
         j = min(f.at, end);
         if (j < f.at) {  // (a rounding away from all that top-k keeps: the bin that it ends in)
@@ -592,6 +606,7 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
         if (filter == 0) all = uniform(all + (double)m.word[1] * kUnit * m.table[j]);
       }
       end = j;
+      lightest = logit_of((uint32_t)(from >> 32));
     }
     __syncthreads();
     if (end < kBins)
@@ -640,6 +655,7 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
   if (least) base = 0.0, part = 0;
   const auto weight_of_token = [&](T logit_of_it, int id) __attribute__((always_inline)) {
     const float l = c.of(logit_of_it);
+    if (l < lightest) return 0.0;
     const Binned b = binned(l, r);
     const int j = c.below(b, l);
     if (j < end || (j == end && j < kBins && order_of(l, id) >= border && (!at_least || heavy(l)))) return weight_of(b) * m.table[j];
