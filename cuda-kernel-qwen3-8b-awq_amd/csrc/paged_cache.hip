@@ -37,9 +37,9 @@ __global__ __launch_bounds__(256) void append_kernel(awq_paged_append_args a, in
   typedef typename Eight<T>::type eight_t;
   const int64_t t = blockIdx.x / blocks;
   const int position = a.positions[t];
-  if (position < 0 || position >= a.max_pos) return;
-  const int dim = a.dim, per_head = dim / 8;
-  const int unit = (int)(blockIdx.x % blocks) * 256 + threadIdx.x, item = unit / per_head, at = (unit % per_head) * 8;
+  const int slot = a.cache ? a.slots[t] : -1;
+  const int dim = a.dim, shift = __builtin_ctz(dim) - 3;  // a head is a power of two
+  const int unit = (int)(blockIdx.x - (uint32_t)t * blocks) * 256 + threadIdx.x, item = unit >> shift, at = (unit & ((1 << shift) - 1)) * 8;
   const int heads = a.q ? a.heads : 0, keys = a.k ? a.kv_heads : 0;
   const bool is_q = item < heads, is_k = !is_q && item < heads + keys;
   const bool is_v = !is_q && !is_k && a.cache && item < heads + 2 * keys;
@@ -49,6 +49,7 @@ __global__ __launch_bounds__(256) void append_kernel(awq_paged_append_args a, in
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = (T)0.0f;
   if (is_q || is_k || is_v) x = *reinterpret_cast<const eight_t*>(src + (int64_t)head * dim + at);
+  if (position < 0 || position >= a.max_pos) return;
   const int half = a.rot / 2;
   const bool turned = (is_q || is_k) && at < a.rot;
   if (a.interleaved) {
@@ -85,9 +86,8 @@ __global__ __launch_bounds__(256) void append_kernel(awq_paged_append_args a, in
   }
   if (is_q) *reinterpret_cast<eight_t*>((T*)a.q_out + t * a.ldq_out + (int64_t)head * dim + at) = x;
   if (is_k && a.k_out) *reinterpret_cast<eight_t*>((T*)a.k_out + t * a.ldk_out + (int64_t)head * dim + at) = x;
-  if (!a.cache) return;
-  const int slot = a.slots[t], page = slot_page(slot, a.n_pages);
-  if (page < 0) return;
+  const int page = slot_page(slot, a.n_pages);
+  if (page < 0 || (!is_k && !is_v)) return;
   float least = INFINITY, largest = -INFINITY, bad = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -121,7 +121,6 @@ __global__ __launch_bounds__(256) void append_kernel(awq_paged_append_args a, in
       word |= (uint32_t)n << (4 * i);
     }
   }
-  if (!is_k && !is_v) return;
   uint8_t* const base = (uint8_t*)a.cache + ((int64_t)page * a.kv_heads + head) * page_head_bytes(dim);
   const int p = slot % kPage, g = at / kGroup;
   if (is_k) {
@@ -150,9 +149,10 @@ __global__ __launch_bounds__(256) void rows_kernel(awq_paged_rows_args a) {
     for (int i = threadIdx.x; i < n; i += 256) starts_of[i] = a.starts[i];
   __syncthreads();
   const int dim = a.dim, half = a.kv_heads * dim / 8, units = ((a.k != nullptr) + (a.v != nullptr)) * half;
-  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x, row = unit / units;
+  // (a 64-bit division takes longer than the rest of a row's eighth)
+  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x, row = gridDim.x < 1u << 24 ? (int64_t)((uint32_t)unit / (uint32_t)units) : unit / units;
   if (row >= a.n_rows) return;
-  const int in_row = (int)(unit % units);
+  const int in_row = (int)(unit - row * units);
   int lo = 0, hi = n;  // the last request that does not start behind the row
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -163,8 +163,8 @@ __global__ __launch_bounds__(256) void rows_kernel(awq_paged_rows_args a) {
   if (row < start || row >= a.starts[lo + 1]) return;
   const int64_t p64 = (a.first ? max(a.first[lo], 0) : 0) + row - start;
   if (p64 >= min(a.lengths[lo], a.max_pages * kPage)) return;
-  const int p = (int)p64, at = in_row % half * 8 % dim, head = in_row % half * 8 / dim;
   const bool value = a.k == nullptr || in_row >= half;
+  const int p = (int)p64, in_heads = (in_row >= half ? in_row - half : in_row) * 8, at = in_heads & (dim - 1), head = in_heads >> __builtin_ctz(dim);
   const int page = held_page(a.table[(int64_t)lo * a.max_pages + p / kPage], a.n_pages);
   eight_t y;
 #pragma unroll
