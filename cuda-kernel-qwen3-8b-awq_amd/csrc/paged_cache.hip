@@ -26,6 +26,21 @@ __device__ __forceinline__ T rounded(double d) {
   return to;
 }
 
+// n s + z in one rounding: a multiply-add of binary16, or the sum of binary32 with the last bit as above (the product is exact, and the sum's
+// rounding error is a number of binary32)
+__device__ __forceinline__ half_t value_of(float n, half_t s, half_t z, half_t) { return __builtin_fmaf16((half_t)n, s, z); }
+__device__ __forceinline__ bf16_t value_of(float n, half_t s, half_t z, bf16_t) {
+  const float a = n * (float)s, b = (float)z;
+  float f = a + b;
+  const float rest = f - a, left = (a - (f - rest)) + (b - rest);
+  if (left != 0.0f) {
+    uint32_t u = __float_as_uint(f);
+    if ((left < 0.0f) != (f < 0.0f)) --u;
+    f = __uint_as_float(u | 1u);
+  }
+  return (bf16_t)f;
+}
+
 constexpr float kHalfMax = 65504.0f;
 
 // A thread takes eight values of a head of a token, so that 64 values with one scale are eight lanes side by side and a head is within
@@ -180,10 +195,10 @@ __global__ __launch_bounds__(256) void rows_kernel(awq_paged_rows_args a) {
       word = *reinterpret_cast<const uint16_t*>(r + value_nibble(dim, at) / 2) |
              (uint32_t)*reinterpret_cast<const uint16_t*>(r + value_nibble(dim, at + 4) / 2) << 16;
     }
-    const double s = (double)(float)*reinterpret_cast<const half_t*>(base + page_parameter(dim, value, g, 0, in_page));
-    const double z = (double)(float)*reinterpret_cast<const half_t*>(base + page_parameter(dim, value, g, 1, in_page));
+    const half_t s = *reinterpret_cast<const half_t*>(base + page_parameter(dim, value, g, 0, in_page));
+    const half_t z = *reinterpret_cast<const half_t*>(base + page_parameter(dim, value, g, 1, in_page));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = rounded<T>((double)((word >> (4 * i)) & 15u) * s + z);
+    for (int i = 0; i < 8; ++i) y[i] = value_of((float)((word >> (4 * i)) & 15u), s, z, T());
   }
   T* const out = value ? (T*)a.v + row * a.ldv : (T*)a.k + row * a.ldk;
   *reinterpret_cast<eight_t*>(out + (int64_t)head * dim + at) = y;
