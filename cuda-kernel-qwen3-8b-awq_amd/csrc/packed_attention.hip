@@ -1,5 +1,6 @@
 // Attention of prompts of different lengths, one behind the other (batch.hpp).
 #include "batch.hpp"
+#include "lane_sums.hpp"
 #include "tile_halves.hpp"
 
 #include <type_traits>
@@ -33,15 +34,14 @@ __device__ __forceinline__ bool find_tile(const awq_packed_attention_args& a, in
   const int lane = threadIdx.x & 63;
   for (int r0 = 0; r0 < a.n_requests; r0 += 64) {
     const int r = r0 + lane;
-    int b = 0, e = 0;
-    if (r < a.n_requests) b = clamped(a.q_starts[r], a.n_tokens), e = clamped(a.q_starts[r + 1], a.n_tokens);
-    const int tiles = e > b ? (e - b + kQueries - 1) / kQueries : 0;
-    int sum = tiles;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int v = __shfl_up(sum, off, 64);
-      if (lane >= off) sum += v;
+    int b = 0, e = 0, kb = 0, ke = 0;
+    const int* const starts = a.k_starts ? a.k_starts : a.q_starts;
+    if (r < a.n_requests) {
+      b = clamped(a.q_starts[r], a.n_tokens), e = clamped(a.q_starts[r + 1], a.n_tokens);
+      kb = clamped(starts[r], a.n_keys), ke = clamped(starts[r + 1], a.n_keys);
     }
+    const int tiles = e > b ? (e - b + kQueries - 1) / kQueries : 0;
+    const int sum = lanes::upto(tiles);
     const int all = __builtin_amdgcn_readlane(sum, 63);
     if (tile < all) {
       const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > tile));
@@ -50,9 +50,8 @@ __device__ __forceinline__ bool find_tile(const awq_packed_attention_args& a, in
       out.q_end = __builtin_amdgcn_readlane(e, at);
       // the last tile first: it has the most keys
       out.first = behind * kQueries;
-      const int* const starts = a.k_starts ? a.k_starts : a.q_starts;
-      out.k_begin = clamped(starts[r0 + at], a.n_keys);
-      out.k_end = clamped(starts[r0 + at + 1], a.n_keys);
+      out.k_begin = __builtin_amdgcn_readlane(kb, at);
+      out.k_end = __builtin_amdgcn_readlane(ke, at);
       return true;
     }
     tile -= all;
