@@ -117,26 +117,27 @@ __global__ __launch_bounds__(256, WAVES) void packed_kernel(awq_packed_attention
   const int row = tid / PIECES, key_part = ((tid % PIECES) ^ key_turn(row)) * 16, value_part = ((tid % PIECES) ^ value_turn(row)) * 16;
   const int64_t key_row = a.ldk * 2, value_row = a.ldv * 2;  // bytes
   const uint32_t key_at = (uint32_t)row * (uint32_t)key_row + key_part, value_at = (uint32_t)row * (uint32_t)value_row + value_part;
-  const auto request = [&](int k0, T* tile) __attribute__((always_inline)) {
-    const uint8_t* kp = (const uint8_t*)kg + k0 * key_row;
-    const uint8_t* vp = (const uint8_t*)vg + k0 * value_row;
+  const auto request = [&](int k0, const T* from, int64_t row_bytes, uint32_t at, int part, T* tile) __attribute__((always_inline)) {
+    const uint8_t* p = (const uint8_t*)from + k0 * row_bytes;
     T* const to = tile + wave * 512;
     if (k0 + kStep <= end) {
 #pragma unroll
-      for (int i = 0; i < P; ++i, kp += kApart * key_row, vp += kApart * value_row) {
-        __builtin_amdgcn_global_load_lds((gptr_t)(kp + key_at), (lptr_t)(to + i * 2048), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((gptr_t)(vp + value_at), (lptr_t)(to + kTile + i * 2048), 16, 0, 0);
-      }
+      for (int i = 0; i < P; ++i, p += kApart * row_bytes) __builtin_amdgcn_global_load_lds((gptr_t)(p + at), (lptr_t)(to + i * 2048), 16, 0, 0);
     } else {  // rows behind the last are masked, and are that one again
 #pragma unroll 1
       for (int i = 0; i < P; ++i) {
-        const uint32_t from = min(row + kApart * i, end - 1 - k0);
-        __builtin_amdgcn_global_load_lds((gptr_t)(kp + (from * (uint32_t)key_row + key_part)), (lptr_t)(to + i * 2048), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((gptr_t)(vp + (from * (uint32_t)value_row + value_part)), (lptr_t)(to + kTile + i * 2048), 16, 0, 0);
+        const uint32_t r = min(row + kApart * i, end - 1 - k0);
+        __builtin_amdgcn_global_load_lds((gptr_t)(p + (r * (uint32_t)row_bytes + part)), (lptr_t)(to + i * 2048), 16, 0, 0);
       }
     }
   };
-  if (end > 0) request(0, tiles);
+  const auto request_keys = [&](int k0, T* tile) __attribute__((always_inline)) { request(k0, kg, key_row, key_at, key_part, tile); };
+  const auto request_values = [&](int k0, T* tile) __attribute__((always_inline)) { request(k0, vg, value_row, value_at, value_part, tile); };
+  if (end > 0) {
+    request_keys(0, tiles);
+    request_values(0, tiles + kTile);
+    if (end > kStep) request_keys(kStep, tiles + 2 * kTile);
+  }
   eight_t qop[D / 16];
   {
     const T* const q = (const T*)a.q + (int64_t)(t.q_begin + qc) * a.ldq + (int64_t)h * D;
@@ -159,22 +160,11 @@ __global__ __launch_bounds__(256, WAVES) void packed_kernel(awq_packed_attention
   float m_run = -INFINITY, l_run = 0.0f;  // (of this lane's keys alone)
   const float mul = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 0x1p-126f);  // (0 times -infinity would be NaN)
 
-  const auto step = [&](int k0, const T* ks) __attribute__((always_inline)) {
-    const T* const vs = ks + kTile;
+  // the scores of a step's keys; s[half][i]: key 32 half + 8 (i / 4) + 4 kh + i % 4
+  const auto score = [&](const T* ks, f32x16_t (&s)[kStep / 32]) __attribute__((always_inline)) {
     int at = lane;
     if constexpr (D == 256) asm volatile("" : "+v"(at));  // addresses in LDS are formed anew each step: there are too many to keep
-    const int L16 = at & 15, n = at & 31, kh = at >> 5;
-    // keys 16 j + 4 kh + L16 / 4 and 8 further, components 32 d + 16 ((lane / 16) % 2) + 4 (L16 % 4) .. + 3
-    const auto values = [&](int j, int d) __attribute__((always_inline)) {
-      const int row = 16 * j + 4 * kh + (L16 >> 2), piece = 4 * d + 2 * ((at >> 4) & 1) + ((L16 >> 1) & 1);
-      const T* const lp = vs + row * D + (piece ^ value_turn(row)) * 8 + (L16 & 1) * 4;
-      const T* const up = vs + (row + 8) * D + (piece ^ value_turn(row + 8)) * 8 + (L16 & 1) * 4;
-      const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4_t __attribute__((address_space(3)))*)lp);
-      const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4_t __attribute__((address_space(3)))*)up);
-      const four_t l4 = __builtin_bit_cast(four_t, lo), u4 = __builtin_bit_cast(four_t, hi);
-      return eight_t{l4[0], l4[1], l4[2], l4[3], u4[0], u4[1], u4[2], u4[3]};
-    };
-    f32x16_t s[kStep / 32];
+    const int n = at & 31, kh = at >> 5;
 #pragma unroll
     for (int half = 0; half < kStep / 32; ++half)
 #pragma unroll
@@ -188,7 +178,23 @@ __global__ __launch_bounds__(256, WAVES) void packed_kernel(awq_packed_attention
         s[half] = product(*reinterpret_cast<const eight_t*>(ks + row * D + ((2 * d + kh) ^ key_turn(row)) * 8), qop[d], s[half]);
       }
     }
-    // s[half][i]: key k0 + 32 half + 8 (i / 4) + 4 kh + i % 4
+  };
+  f32x16_t s[kStep / 32];
+  // the step at k0, whose scores are there; `ks`: the next one's keys
+  const auto step = [&](int k0, const T* ks, const T* vs) __attribute__((always_inline)) {
+    int at = lane;
+    if constexpr (D == 256) asm volatile("" : "+v"(at));
+    const int L16 = at & 15, kh = at >> 5;
+    // keys 16 j + 4 kh + L16 / 4 and 8 further, components 32 d + 16 ((lane / 16) % 2) + 4 (L16 % 4) .. + 3
+    const auto values = [&](int j, int d) __attribute__((always_inline)) {
+      const int row = 16 * j + 4 * kh + (L16 >> 2), piece = 4 * d + 2 * ((at >> 4) & 1) + ((L16 >> 1) & 1);
+      const T* const lp = vs + row * D + (piece ^ value_turn(row)) * 8 + (L16 & 1) * 4;
+      const T* const up = vs + (row + 8) * D + (piece ^ value_turn(row + 8)) * 8 + (L16 & 1) * 4;
+      const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4_t __attribute__((address_space(3)))*)lp);
+      const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4_t __attribute__((address_space(3)))*)up);
+      const four_t l4 = __builtin_bit_cast(four_t, lo), u4 = __builtin_bit_cast(four_t, hi);
+      return eight_t{l4[0], l4[1], l4[2], l4[3], u4[0], u4[1], u4[2], u4[3]};
+    };
     if (k0 + kStep > least) {
       const int sees = seen - k0 - 4 * kh;
 #pragma unroll
@@ -216,29 +222,66 @@ __global__ __launch_bounds__(256, WAVES) void packed_kernel(awq_packed_attention
     move_maximum<true>(mx > -INFINITY ? mx * scale : -INFINITY, m_run, l_run, o);
     const float from = m_run == -INFINITY ? 0.0f : m_run;  // (no key seen yet: all weights are 0)
     eight_t pop[kStep / 16];
+    const auto weights = [&](int first, int many) __attribute__((always_inline)) {  // of the lane's kStep / 2 scores
+#pragma unroll
+      for (int x = first; x < first + many; ++x) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x / 16][x % 16], scale, -from));
+        l_run += p;
+        pop[x / 8][x % 8] = (T)p;
+      }
+    };
+    // A few weights behind each of the next scores' products, which take as long; behind the last step these are of what lies there, and unused
+    f32x16_t next[kStep / 32];
 #pragma unroll
     for (int half = 0; half < kStep / 32; ++half)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[half][i], scale, -from));
-        l_run += p;
-        pop[2 * half + (i >> 3)][i & 7] = (T)p;
-      }
+      for (int i = 0; i < 16; ++i) next[half][i] = 0.0f;
+    const auto key = [&](int d, int half) __attribute__((always_inline)) {
+      const int row = 32 * half + (at & 31);
+      return *reinterpret_cast<const eight_t*>(ks + row * D + ((2 * d + kh) ^ key_turn(row)) * 8);
+    };
+    constexpr int HALVES = kStep / 32, ROUNDS = D / 16, EACH = kStep / 2 / ROUNDS;
+    static_assert(ROUNDS * EACH == kStep / 2, "all weights");
+    eight_t ahead[HALVES];
 #pragma unroll
-    for (int j = 0; j < kStep / 16; ++j)
+    for (int half = 0; half < HALVES; ++half) ahead[half] = key(0, half);
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d) {
-        if (D == 256 && d % 4 == 0) __builtin_amdgcn_sched_barrier(0);
-        o[d] = product(values(j, d), pop[j], o[d]);
+    for (int d = 0; d < ROUNDS; ++d) {
+      eight_t now[HALVES];
+#pragma unroll
+      for (int half = 0; half < HALVES; ++half) now[half] = ahead[half];
+      if (d + 1 < ROUNDS)
+#pragma unroll
+        for (int half = 0; half < HALVES; ++half) ahead[half] = key(d + 1, half);
+#pragma unroll
+      for (int half = 0; half < HALVES; ++half) {
+        next[half] = product(now[half], qop[d], next[half]);
+        weights(d * EACH + half * (EACH / HALVES), EACH / HALVES);
+        __builtin_amdgcn_sched_barrier(0);
       }
+    }
+#pragma unroll
+    for (int half = 0; half < HALVES; ++half) s[half] = next[half];
+    constexpr int PRODUCTS = kStep / 16 * (D / 32), AHEAD = 2;
+    eight_t v[PRODUCTS];
+#pragma unroll
+    for (int x = 0; x < AHEAD; ++x) v[x] = values(x / (D / 32), x % (D / 32));
+#pragma unroll
+    for (int x = 0; x < PRODUCTS; ++x) {
+      if (x + AHEAD < PRODUCTS) v[x + AHEAD] = values((x + AHEAD) / (D / 32), (x + AHEAD) % (D / 32));
+      o[x % (D / 32)] = product(v[x], pop[x / (D / 32)], o[x % (D / 32)]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
   const int unmasked = seen_by(min(t.first, nq - 1));  // keys that all queries of the workgroup see
-  T* ks = tiles;
+  __syncthreads();
+  if (end > 0) score(tiles, s);
+  T *here = tiles, *other = tiles + 2 * kTile;  // this step's keys and values, the next one's
   for (int k0 = 0; k0 < end; k0 += kStep) {
-    __syncthreads();  // these keys and values are there, the last ones' readers done
+    __syncthreads();  // the next keys and these values are there, the last ones' readers done
     bool strange = false;
     if (k0 + kStep > unmasked) {
-      u32x4_t* const vs = reinterpret_cast<u32x4_t*>(ks + kTile) + tid;
+      u32x4_t* const vs = reinterpret_cast<u32x4_t*>(here + kTile) + tid;
       uint32_t any = 0;
 #pragma unroll
       for (int i = 0; i < P; ++i) any |= not_finite<T>(vs[256 * i]);
@@ -249,9 +292,9 @@ __global__ __launch_bounds__(256, WAVES) void packed_kernel(awq_packed_attention
         __syncthreads();
       }
     }
-    T* const other = tiles + (ks == tiles ? 2 * kTile : 0);
-    if (k0 + kStep < end) request(k0 + kStep, other);
-    if (k0 < most) step(k0, ks);
+    if (k0 + 2 * kStep < end) request_keys(k0 + 2 * kStep, here);
+    if (k0 + kStep < end) request_values(k0 + kStep, other + kTile);
+    if (k0 < most) step(k0, other, here + kTile);
     if (strange) {
 #pragma unroll 1
       for (int key = k0; key < min(k0 + kStep, most); ++key) {
@@ -267,7 +310,9 @@ __global__ __launch_bounds__(256, WAVES) void packed_kernel(awq_packed_attention
         }
       }
     }
-    ks = other;
+    T* const last = here;
+    here = other;
+    other = last;
   }
   if (qi >= nq) return;
   const HalfPair sums = half_pair(l_run);
