@@ -230,38 +230,41 @@ __global__ __launch_bounds__(256, WAVES) void packed_kernel(awq_packed_attention
         pop[x / 8][x % 8] = (T)p;
       }
     };
-    // A few weights behind each of the next scores' products, which take as long; behind the last step these are of what lies there, and unused
-    f32x16_t next[kStep / 32];
-#pragma unroll
-    for (int half = 0; half < kStep / 32; ++half)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) next[half][i] = 0.0f;
-    const auto key = [&](int d, int half) __attribute__((always_inline)) {
-      const int row = 32 * half + (at & 31);
-      return *reinterpret_cast<const eight_t*>(ks + row * D + ((2 * d + kh) ^ key_turn(row)) * 8);
-    };
     constexpr int HALVES = kStep / 32, ROUNDS = D / 16, EACH = kStep / 2 / ROUNDS;
     static_assert(ROUNDS * EACH == kStep / 2, "all weights");
-    eight_t ahead[HALVES];
+    if (k0 + kStep < most) {  // a few weights behind each of the next scores' products, which take as long
+      f32x16_t next[kStep / 32];
 #pragma unroll
-    for (int half = 0; half < HALVES; ++half) ahead[half] = key(0, half);
+      for (int half = 0; half < kStep / 32; ++half)
 #pragma unroll
-    for (int d = 0; d < ROUNDS; ++d) {
-      eight_t now[HALVES];
+        for (int i = 0; i < 16; ++i) next[half][i] = 0.0f;
+      const auto key = [&](int d, int half) __attribute__((always_inline)) {
+        const int row = 32 * half + (at & 31);
+        return *reinterpret_cast<const eight_t*>(ks + row * D + ((2 * d + kh) ^ key_turn(row)) * 8);
+      };
+      eight_t ahead[HALVES];
 #pragma unroll
-      for (int half = 0; half < HALVES; ++half) now[half] = ahead[half];
-      if (d + 1 < ROUNDS)
+      for (int half = 0; half < HALVES; ++half) ahead[half] = key(0, half);
 #pragma unroll
-        for (int half = 0; half < HALVES; ++half) ahead[half] = key(d + 1, half);
+      for (int d = 0; d < ROUNDS; ++d) {
+        eight_t now[HALVES];
 #pragma unroll
-      for (int half = 0; half < HALVES; ++half) {
-        next[half] = product(now[half], qop[d], next[half]);
-        weights(d * EACH + half * (EACH / HALVES), EACH / HALVES);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int half = 0; half < HALVES; ++half) now[half] = ahead[half];
+        if (d + 1 < ROUNDS)
+#pragma unroll
+          for (int half = 0; half < HALVES; ++half) ahead[half] = key(d + 1, half);
+#pragma unroll
+        for (int half = 0; half < HALVES; ++half) {
+          next[half] = product(now[half], qop[d], next[half]);
+          weights(d * EACH + half * (EACH / HALVES), EACH / HALVES);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
-    }
 #pragma unroll
-    for (int half = 0; half < HALVES; ++half) s[half] = next[half];
+      for (int half = 0; half < HALVES; ++half) s[half] = next[half];
+    } else {
+      weights(0, kStep / 2);
+    }
     constexpr int PRODUCTS = kStep / 16 * (D / 32), AHEAD = 2;
     eight_t v[PRODUCTS];
 #pragma unroll
@@ -334,7 +337,7 @@ int launch(const awq_packed_attention_args& a, hipStream_t st) {
   const int64_t tiles = a.n_tokens / kQueries + std::min<int64_t>(a.n_requests, a.n_tokens);
   AWQ_REQUIRE(tiles * a.heads < (1ll << 31), "too many queries and heads");
   const dim3 grid((unsigned)(tiles * a.heads));
-  if (a.dim == 64) hipLaunchKernelGGL((packed_kernel<T, 64, 64, 3>), grid, dim3(256), 0, st, a);
+  if (a.dim == 64) hipLaunchKernelGGL((packed_kernel<T, 64, 64, 2>), grid, dim3(256), 0, st, a);
   else if (a.dim == 128) hipLaunchKernelGGL((packed_kernel<T, 128, 64, 2>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((packed_kernel<T, 256, 64, 1>), grid, dim3(256), 0, st, a);
   AWQ_HIP_TRY(hipGetLastError());
