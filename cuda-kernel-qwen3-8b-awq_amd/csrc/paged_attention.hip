@@ -12,11 +12,16 @@ typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4;     // of a workgroup, each with pages of its own
 constexpr int kColumns = 16;  // query heads of one key/value head that share a pass over the pages
 
+// Wavefronts of a SIMD: as many as have all their numbers in registers.  Heads of 128, 64 requests of 8 key/value heads with 4 query heads each:
+// 4 (some numbers in scratch memory) 49 us, 3 42, 2 44; 2 key/value heads with 16: 4 37 us, 2 20; heads of 256 with 16: 2 39 us, 1 25.
+constexpr int resident(int dim, int columns) {
+  return dim == 64 ? (columns > 8 ? 2 : 4) : dim == 128 ? (columns > 8 ? 2 : 3) : (columns > 8 ? 1 : 2);
+}
 inline int columns_of(int group) { return std::min(group, kColumns); }
 inline int streams_of(int heads, int kv_heads) { return kv_heads * ((heads / kv_heads + kColumns - 1) / kColumns); }
-// wavefronts that share the pages of a stream (a key/value head and up to 16 of its query heads): as many as the chip holds with a page each in LDS
+// wavefronts that share the pages of a stream (a key/value head and up to 16 of its query heads): as many as the chip holds, each with a page in LDS
 inline int workers_of(int n_requests, int heads, int kv_heads, int dim, int max_pages) {
-  const int64_t there = 256ll * (dim == 256 ? 8 : 16) / streams_of(heads, kv_heads);
+  const int64_t there = 1024ll * resident(dim, heads / kv_heads) / streams_of(heads, kv_heads);
   const int64_t most = (int64_t)n_requests * max_pages;
   return (int)std::max<int64_t>(kWaves, (std::min(there, most) + kWaves - 1) / kWaves * kWaves);
 }
@@ -77,7 +82,7 @@ __device__ __forceinline__ int run_of(int all, int workers) { return (all + work
 // Weights are relative to the largest of score + exponent of the page's largest value scale, so that p s is below 1 and as exact as
 // binary16 can be whatever the values' size.
 template <typename T, int D, int COLUMNS>
-__global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 4) void paged_kernel(PagedArgs p) {
+__global__ __launch_bounds__(64 * kWaves, resident(D, COLUMNS)) void paged_kernel(PagedArgs p) {
   constexpr int G = D / 64, PIECES = D / 32;  // groups; 16-byte pieces of a row
   constexpr int TP = 16 / COLUMNS, SETS = 4 / TP;
   constexpr int kBytes = 72 * D, kKeyLoads = D / 32 + (D + 127) / 128, kValueLoads = D / 32;
