@@ -86,7 +86,7 @@ __device__ __forceinline__ u32x4_t only_finite(u32x4_t v) {
 // A row's 16-byte pieces lie rotated in LDS so that the rows that lanes read together are in all banks.
 // A step's scores are formed during the step ahead, each product of theirs beside a few of its weights, so that matrix and vector instructions of one
 // wavefront run together; keys are therefore requested two steps ahead, values one.
-// Heads of 128, 32 over 8: 13 prompts of 60 to 1,000 tokens, binary16, 50 us; 3 parts of 500 to 1,100 tokens behind 3,500 each, bfloat16, 188 us, 680 TFLOP/s.
+// Heads of 128, 32 over 8: 13 prompts of 60 to 1,000 tokens, binary16, 50 us; 3 parts of 500 to 1,100 tokens behind 3,500 each, bfloat16, 188 us, 0.71 PFLOP/s.
 // Bound by the two kinds of instructions (each a third of the time) and by 800 workgroups on 512 places.  64 keys a step and two wavefronts a
 // SIMD: 32 keys and three 57 and 236 us where these took 54 and 216; scores in their own step 53 and 206 where they now take 50 and 188.
 // Where some query of the workgroup does not see all keys of a step, values that are not finite are kept out of the product, in which 0 times

@@ -169,7 +169,7 @@ __global__ __launch_bounds__(kSlotThreads) void slots_kernel(awq_page_plan_args 
 
 }  // namespace
 
-// One launch or two: 200 requests with a position each 9.0 us in one, 8.1 + 2.1 in two; 240 requests with 8,400 positions 17.1 us in one, 8.3 + 3.5 in two.
+// One launch or two: 200 requests with a position each 9.0 us in one, 8.1 + 2.1 in two; 240 requests with 10,800 positions 17.1 us in one, 8.3 + 3.5 in two.
 int launch_page_plan(const awq_page_plan_args& a, hipStream_t st) {
   if (a.n_requests <= kPlanThreads && a.max_tokens <= kPlanTokens) {
     hipLaunchKernelGGL(plan_kernel<true>, dim3(1), dim3(kPlanThreads), 0, st, a);

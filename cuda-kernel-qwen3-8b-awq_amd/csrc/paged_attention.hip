@@ -80,7 +80,7 @@ __device__ __forceinline__ int run_of(int all, int workers) { return (all + work
 // so are the sums of the values' pieces), so that a word of eight takes five instructions.  The scales are put on afterwards: on a key's
 // sum over a group, s sum(q n) + z sum(q) in binary32, and on the weights, p s rounded to binary16 for the product, p z in binary32.
 // Heads of 128, 32 over 8: 64 requests of 100 to 8,000 positions, bfloat16, 42 us, 4.2 TB/s of the cache; one of 40,960 positions, binary16, 17 us (its
-// 640 pages leave a worker two or three); 12 requests of 5 to 300 positions, 16 heads of 64, 6 us.  Bound by memory and, at a few pages a worker, by the start.
+// 640 pages leave a worker two); 12 requests of 5 to 300 positions, 16 heads of 64, 6 us.  Bound by memory and, at a few pages a worker, by the start.
 // Weights are relative to the largest of score + exponent of the page's largest value scale, so that p s is below 1 and as exact as
 // binary16 can be whatever the values' size.
 template <typename T, int D, int COLUMNS>
