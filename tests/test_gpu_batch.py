@@ -806,3 +806,70 @@ def test_calls_on_streams_of_their_own(dev):
             dev.awq.check(dev.lib.awq_sample(ctypes.byref(args), 3, ctypes.c_void_p(st.cuda_stream)))
     for (ctx, ids, _, _), (want, want_ids) in zip(outs, alone):
         assert np.array_equal(dev.host(ctx), want) and dev.host(ids).tolist() == want_ids
+
+
+def test_captured_parts_of_prompts(dev):
+    """passes of three requests with 5, 1 and 30 new positions each, behind what they have, as a graph that is replayed: the ids of the same passes
+    run one by one"""
+    torch, new = dev.torch, [5, 1, 30]
+    runs = []
+    for captured in (False, True):
+        rng = rng_of(13)
+        s = Server(dev, "bf16")
+        s.start(3)
+        u, fresh, tokens, got = dev.floats([0.0] * 3), dev.ints(new), dev.ints([0] * 40), []
+        state = (s.lengths, s.count, s.table, s.ids, s.cache)
+        graph = None
+        if captured:
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            saved = [t.clone() for t in state]
+            with torch.cuda.stream(side):
+                s.step(tokens, fresh, True, u, 40)
+            torch.cuda.current_stream().wait_stream(side)
+            torch.cuda.synchronize()
+            for t, was in zip(state, saved):
+                t.copy_(was)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                s.step(tokens, fresh, True, u, 40)
+        for _ in range(6):
+            u.copy_(dev.floats(rng.random(3)))
+            tokens.copy_(dev.ints(rng.integers(0, s.vocab, 40)))
+            if graph is not None:
+                graph.replay()
+            else:
+                s.step(tokens, fresh, True, u, 40)
+            got.append(dev.host(s.ids).tolist())
+            (torch.ones(1000, device="cuda") * 2).sum().item()
+        runs.append((got, dev.host(s.lengths).tolist(), dev.host(s.cache).tobytes()))
+    assert runs[0][1] == [30, 6, 180] and runs[0] == runs[1]
+
+
+def test_packed_attention_of_rows_far_apart(dev):
+    """strides with which rows lie further than 2^32 bytes from the first"""
+    heads, kv, dim, new = 2, 1, 128, [100, 64]
+    rng, n, ld = rng_of(14), 164, (1 << 24) + 8
+    print("rows far apart", flush=True)
+    x = dev.torch.empty((n, ld), dtype=dev.torch.float16, device="cuda")
+    d_y, vy = dev.act(rng.standard_normal((n, (heads + 2 * kv) * dim)), "f16")
+    x[:, :d_y.shape[1]] = d_y
+    ctx = x[:, 1024:1024 + heads * dim]
+    ctx.fill_(9.0)
+    starts = np.cumsum([0] + new)
+    got = packed(dev, "f16", x, x[:, heads * dim:], x[:, (heads + kv) * dim:], starts, None, heads, kv, dim, True, dim ** -0.5, ctx)
+    parts = [vy[:, a * dim:b * dim].reshape(n, b - a, dim) for a, b in ((0, heads), (heads, heads + kv), (heads + kv, heads + 2 * kv))]
+    check_packed(got.reshape(n, heads, dim), "f16", *parts, starts, starts, True, dim ** -0.5)
+
+
+def test_sample_of_the_largest_vocabulary_and_of_rows_far_apart(dev):
+    V, n = 524288, 3
+    rng, ld = rng_of(15), (1 << 30) + 8
+    print("largest vocabulary", flush=True)
+    d_x, vx = dev.act(2.0 * rng.standard_normal((n, V)), "f16")
+    x = dev.torch.empty((n, ld), dtype=dev.torch.float16, device="cuda")
+    x[:, :V] = d_x
+    u = rng.random(n).astype(np.float32)
+    for t, k, p, m in ((None, None, None, None), ([0.0] * n, None, None, None), ([0.7, 1.0, 1.4], [50, 4000, 300000], None, None), ([1.0, 0.5, 1.3], None, [0.9, 0.99, 0.95], None),
+                       (None, [400] * n, [0.9] * n, [0.02] * n)):
+        check_sample(dev, "f16", vx, sample(dev, "f16", x, u, t, k, p, m, V), u, t, k, p, m)
