@@ -46,8 +46,8 @@ constexpr float kHalfMax = 65504.0f;
 // A thread takes eight values of a head of a token, so that 64 values with one scale are eight lanes side by side and a head is within
 // a wavefront.  Everything behind the load is in 64 bits, in which the turned values are exact: a value next to a border of the
 // number format, and a quotient next to a half, then go where the formula sends them.
-// 8,000 positions of 32 + 8 heads of 128, 64 of them turned, bfloat16: 60 us, 3.2 TB/s of what it reads and writes (190 MB); vector instructions fill
-// three quarters of that time.  64 positions: 4 us, a launch.
+// 8,000 positions of 32 + 8 heads of 128, 64 of them turned, bfloat16: 55 us, 3.5 TB/s of what it reads and writes (190 MB), beside vector
+// instructions for most of that time.  64 positions: 4 us, a launch.
 template <typename T>
 __global__ __launch_bounds__(256) void append_kernel(awq_paged_append_args a, int blocks) {
   typedef typename Eight<T>::type eight_t;
@@ -55,8 +55,18 @@ __global__ __launch_bounds__(256) void append_kernel(awq_paged_append_args a, in
   const int position = a.positions[t];
   const int slot = a.cache ? a.slots[t] : -1;
   const int dim = a.dim, shift = __builtin_ctz(dim) - 3;  // a head is a power of two
-  const int unit = (int)(blockIdx.x - (uint32_t)t * blocks) * 256 + threadIdx.x, item = unit >> shift, at = (unit & ((1 << shift) - 1)) * 8;
+  const int unit = (int)(blockIdx.x - (uint32_t)t * blocks) * 256 + threadIdx.x;
   const int heads = a.q ? a.heads : 0, keys = a.k ? a.kv_heads : 0;
+  int item = unit >> shift, at = (unit & ((1 << shift) - 1)) * 8;
+  if (a.rot <= kGroup) {
+    // all heads' first 64 values, then the next: a wavefront's lanes are turned together or not at all (half of heads of 128 turned: 55 us, head by head
+    // 60; with more than 64 turned a pair may lie in two of these parts)
+    const int items = heads + (a.cache ? 2 : 1) * keys, groups = dim / kGroup;
+    item = unit >> 3;
+    at = (unit & 7) * 8;
+    for (int g = 1; g < groups; ++g)
+      if (item >= items) item -= items, at += kGroup;
+  }
   const bool is_q = item < heads, is_k = !is_q && item < heads + keys;
   const bool is_v = !is_q && !is_k && a.cache && item < heads + 2 * keys;
   const int head = is_q ? item : is_k ? item - heads : item - heads - keys;
@@ -80,7 +90,7 @@ __global__ __launch_bounds__(256) void append_kernel(awq_paged_append_args a, in
         x[2 * i + 1] = rounded<T>(u * sd + v * cd);
       }
     }
-  } else if (a.rot) {
+  } else if (a.rot && __builtin_amdgcn_ballot_w64(turned)) {
     // the other halves of the pairs are half / 8 lanes away; they are exchanged ahead of any store, so that q_out may be q
     const bool first = at < half;
     const int other = (int)(threadIdx.x & 63) + (turned ? (first ? half / 8 : -half / 8) : 0);
