@@ -24,18 +24,20 @@ __device__ __forceinline__ f32x16_t product(Vec<bf16_t>::eight a, Vec<bf16_t>::e
 }
 constexpr int kQueries = 128;
 
-// The tile of queries a workgroup takes: request r has ceil(queries / 128) of them, tiles are numbered one request behind the other. Every
-// wavefront looks its own up, 64 requests at a time.  False: there are fewer tiles.
+// The tile of queries a workgroup takes: request r has ceil(queries / 128) of them.  Every wavefront looks its own up.  False: there are fewer tiles.
+// Up to 64 requests, a lane each: tiles with the most keys first, by 128 keys; what runs last is short.  (13 prompts of 60 to 1,000 tokens, one request
+// behind the other 50 us, so 47; 3 parts of long prompts, all long, 188 and 189.)  More requests: one behind the other, 64 at a time, the last tile of each first, which has
+// the most keys; the search would read them all some ten times.
 struct Tile {
   int q_begin, q_end, k_begin, k_end, first;  // first: of the tile's queries, from q_begin on
 };
 __device__ __forceinline__ int clamped(int64_t x, int64_t n) { return (int)(x < 0 ? 0 : x > n ? n : x); }
 __device__ __forceinline__ bool find_tile(const awq_packed_attention_args& a, int tile, Tile& out) {
   const int lane = threadIdx.x & 63;
+  const int* const starts = a.k_starts ? a.k_starts : a.q_starts;
   for (int r0 = 0; r0 < a.n_requests; r0 += 64) {
     const int r = r0 + lane;
     int b = 0, e = 0, kb = 0, ke = 0;
-    const int* const starts = a.k_starts ? a.k_starts : a.q_starts;
     if (r < a.n_requests) {
       b = clamped(a.q_starts[r], a.n_tokens), e = clamped(a.q_starts[r + 1], a.n_tokens);
       kb = clamped(starts[r], a.n_keys), ke = clamped(starts[r + 1], a.n_keys);
@@ -43,6 +45,31 @@ __device__ __forceinline__ bool find_tile(const awq_packed_attention_args& a, in
     const int tiles = e > b ? (e - b + kQueries - 1) / kQueries : 0;
     const int sum = lanes::upto(tiles);
     const int all = __builtin_amdgcn_readlane(sum, 63);
+    if (a.n_requests <= 64) {
+      if (tile >= all) return false;
+      // A request's tiles from the last on are at the levels top, top - 1, .. (all at top where all see all keys), those without keys at 0.
+      const int nk = max(ke - kb, 0), top = (a.causal ? max(nk - (e - b - (tiles - 1) * kQueries), 0) : nk) / kQueries + 1;
+      const auto from_level = [&](int level) __attribute__((always_inline)) {  // tiles at it or above
+        return level <= 0 ? tiles : a.causal ? min(max(top - level + 1, 0), tiles) : level <= top ? tiles : 0;
+      };
+      const auto over_all = [](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(lanes::upto(v), 63); };
+      // the level of the tile: the highest with more tiles from it on than are ahead of this one
+      int lo = 0, hi = __builtin_amdgcn_readfirstlane((int)lanes::maximum<64>(tiles ? (float)top : 0.0f));  // (at most 2^24: exact)
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (over_all(from_level(mid)) > tile) lo = mid;
+        else hi = mid - 1;
+      }
+      const int above = from_level(lo + 1), here = from_level(lo) - above, upto = lanes::upto(here), rest = tile - over_all(above);
+      const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > rest) | 1ull << 63);
+      const int behind = __builtin_amdgcn_readlane(above, at) + rest - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(here, at));
+      out.q_begin = __builtin_amdgcn_readlane(b, at);
+      out.q_end = __builtin_amdgcn_readlane(e, at);
+      out.first = (__builtin_amdgcn_readlane(tiles, at) - 1 - behind) * kQueries;
+      out.k_begin = __builtin_amdgcn_readlane(kb, at);
+      out.k_end = __builtin_amdgcn_readlane(ke, at);
+      return true;
+    }
     if (tile < all) {
       const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > tile));
       const int behind = __builtin_amdgcn_readlane(sum, at) - 1 - tile;  // tiles of the request behind this one
@@ -86,7 +113,7 @@ __device__ __forceinline__ u32x4_t only_finite(u32x4_t v) {
 // A row's 16-byte pieces lie rotated in LDS so that the rows that lanes read together are in all banks.
 // A step's scores are formed during the step ahead, each product of theirs beside a few of its weights, so that matrix and vector instructions of one
 // wavefront run together; keys are therefore requested two steps ahead, values one.
-// Heads of 128, 32 over 8: 13 prompts of 60 to 1,000 tokens, binary16, 50 us; 3 parts of 500 to 1,100 tokens behind 3,500 each, bfloat16, 188 us, 0.71 PFLOP/s.
+// Heads of 128, 32 over 8: 13 prompts of 60 to 1,000 tokens, binary16, 47 us; 3 parts of 500 to 1,100 tokens behind 3,500 each, bfloat16, 188 us, 0.71 PFLOP/s.
 // Bound by the two kinds of instructions (each a third of the time) and by 800 workgroups on 512 places.  64 keys a step and two wavefronts a
 // SIMD: 32 keys and three 57 and 236 us where these took 54 and 216; scores in their own step 53 and 206 where they now take 50 and 188.
 // Where some query of the workgroup does not see all keys of a step, values that are not finite are kept out of the product, in which 0 times
