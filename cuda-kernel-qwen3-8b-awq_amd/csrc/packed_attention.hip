@@ -113,9 +113,10 @@ __device__ __forceinline__ u32x4_t only_finite(u32x4_t v) {
 // A row's 16-byte pieces lie rotated in LDS so that the rows that lanes read together are in all banks.
 // A step's scores are formed during the step ahead, each product of theirs beside a few of its weights, so that matrix and vector instructions of one
 // wavefront run together; keys are therefore requested two steps ahead, values one.
-// Heads of 128, 32 over 8: 13 prompts of 60 to 1,000 tokens, binary16, 47 us; 3 parts of 500 to 1,100 tokens behind 3,500 each, bfloat16, 188 us, 0.71 PFLOP/s.
+// Heads of 128, 32 over 8: 13 prompts of 60 to 1,000 tokens, binary16, 46 us; 3 parts of 500 to 1,100 tokens behind 3,500 each, bfloat16, 179 us, 0.74 PFLOP/s.
 // Bound by the two kinds of instructions (each a third of the time) and by 800 workgroups on 512 places.  64 keys a step and two wavefronts a
-// SIMD: 32 keys and three 57 and 236 us where these took 54 and 216; scores in their own step 53 and 206 where they now take 50 and 188.
+// SIMD: 32 keys and three 57 and 236 us where these took 54 and 216; scores in their own step 53 and 206, formed a step ahead 50 and 188 (and 47 and 179 with the first values
+// read ahead of them); heads of 64 with three wavefronts, some numbers in scratch memory, 74 us, with two 72.
 // Where some query of the workgroup does not see all keys of a step, values that are not finite are kept out of the product, in which 0 times
 // them is NaN, and are added for the queries that see them.
 template <typename T, int D, int kStep, int WAVES>
@@ -264,6 +265,10 @@ __global__ __launch_bounds__(256, WAVES) void packed_kernel(awq_packed_attention
     };
     constexpr int HALVES = kStep / 32, ROUNDS = D / 16, EACH = kStep / 2 / ROUNDS;
     static_assert(ROUNDS * EACH == kStep / 2, "all weights");
+    constexpr int PRODUCTS = kStep / 16 * (D / 32), AHEAD = 2;
+    eight_t v[PRODUCTS];
+#pragma unroll
+    for (int x = 0; x < AHEAD; ++x) v[x] = values(x / (D / 32), x % (D / 32));
     if (k0 + kStep < most) {  // a few weights behind each of the next scores' products, which take as long
       f32x16_t next[kStep / 32];
 #pragma unroll
@@ -297,10 +302,6 @@ __global__ __launch_bounds__(256, WAVES) void packed_kernel(awq_packed_attention
     } else {
       weights(0, kStep / 2);
     }
-    constexpr int PRODUCTS = kStep / 16 * (D / 32), AHEAD = 2;
-    eight_t v[PRODUCTS];
-#pragma unroll
-    for (int x = 0; x < AHEAD; ++x) v[x] = values(x / (D / 32), x % (D / 32));
 #pragma unroll
     for (int x = 0; x < PRODUCTS; ++x) {
       if (x + AHEAD < PRODUCTS) v[x + AHEAD] = values((x + AHEAD) / (D / 32), (x + AHEAD) % (D / 32));
