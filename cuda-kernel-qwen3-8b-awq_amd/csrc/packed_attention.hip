@@ -112,7 +112,8 @@ __device__ __forceinline__ u32x4_t only_finite(u32x4_t v) {
 // are binary32; a weight is rounded to the activations' type for the second product alone.
 // A row's 16-byte pieces lie rotated in LDS so that the rows that lanes read together are in all banks.
 // A step's scores are formed during the step ahead, each product of theirs beside a few of its weights, so that matrix and vector instructions of one
-// wavefront run together; keys are therefore requested two steps ahead, values one.
+// wavefront run together; keys are therefore requested two steps ahead, values one.  (What is on its way is waited for ahead of a step's first
+// transposing read, the compiler's doing, and ahead of the next barrier: a request runs beside the step's masks and maximum.)
 // Heads of 128, 32 over 8: 13 prompts of 60 to 1,000 tokens, binary16, 46 us; 3 parts of 500 to 1,100 tokens behind 3,500 each, bfloat16, 179 us, 0.74 PFLOP/s.
 // Bound by the two kinds of instructions (each a third of the time) and by 800 workgroups on 512 places.  64 keys a step and two wavefronts a
 // SIMD: 32 keys and three 57 and 236 us where these took 54 and 216; scores in their own step 53 and 206, formed a step ahead 50 and 188 (and 47 and 179 with the first values
@@ -310,11 +311,16 @@ __global__ __launch_bounds__(256, WAVES) void packed_kernel(awq_packed_attention
     }
   };
   const int unmasked = seen_by(min(t.first, nq - 1));  // keys that all queries of the workgroup see
-  __syncthreads();
+  // A barrier does not wait for requests into LDS: every wavefront waits for its own ahead of it, also one without products in a step.
+  const auto all_there = []() __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  all_there();
   if (end > 0) score(tiles, s);
   T *here = tiles, *other = tiles + 2 * kTile;  // this step's keys and values, the next one's
   for (int k0 = 0; k0 < end; k0 += kStep) {
-    __syncthreads();  // the next keys and these values are there, the last ones' readers done
+    all_there();  // the next keys and these values, and the last ones' readers are done
     bool strange = false;
     if (k0 + kStep > unmasked) {
       u32x4_t* const vs = reinterpret_cast<u32x4_t*>(here + kTile) + tid;

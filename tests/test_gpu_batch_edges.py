@@ -1,0 +1,50 @@
+"""Several requests at once: what lies at the edges of the operators' definitions, against batch_plain.py's 64 bits."""
+import numpy as np
+import pytest
+
+import batch_plain as plain
+from test_gpu_batch import dev, packed, rng_of  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# --- attention of packed prompts ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("behind", [32, 96, 160])
+def test_packed_attention_beside_what_is_not_finite_in_a_step_that_some_wavefronts_skip(dev, dtype, dim, behind):
+    """Requests with positions ahead of their queries: the first wavefronts of a tile are done some steps ahead of the last ones, and all of them look
+    for values that are not finite.  Those of keys that a query does not see do not reach it, those of keys it sees do."""
+    heads, kv, new = 2, 1, [150, 128, 200, 129]
+    rng = rng_of(dtype, dim, behind)
+    print("packed, not finite", dtype, dim, behind, flush=True)
+    q_starts, k_starts = np.cumsum([0] + new), np.cumsum([0] + [n + behind for n in new])
+    n_q, n_k = int(q_starts[-1]), int(k_starts[-1])
+    d_q, vq = dev.act(rng.standard_normal((n_q, heads * dim)), dtype)
+    d_k, vk = dev.act(rng.standard_normal((n_k, kv * dim)), dtype)
+    v = rng.standard_normal((n_k, kv * dim))
+    for c in k_starts[:-1]:
+        v[c + behind + 97, 0], v[c + behind + 99, 7], v[c + behind + 127, dim - 1] = -np.inf, np.inf, np.nan
+    d_v, vv = dev.act(v, dtype)
+    got = packed(dev, dtype, d_q, d_k, d_v, q_starts, k_starts, heads, kv, dim, True, dim ** -0.5, dev.full((n_q, heads * dim), 9.0, dtype))
+    got = got.reshape(n_q, heads, dim)
+    finite = np.where(np.isfinite(vv), vv, 0.0)
+    for a, c, n in zip(q_starts, k_starts, new):
+        at = np.arange(n)
+        for first, column, want in ((97, 0, -np.inf), (99, 7, np.inf), (127, dim - 1, np.nan)):
+            x = got[a:a + n, :, column]
+            assert np.isfinite(x[at < first]).all()
+            assert np.isnan(x[at >= first]).all() if np.isnan(want) else (x[at >= first] == want).all()
+            got[a:a + n, :, column][at >= first] = 0.0
+    # the columns without them are those of finite values, and so are the queries ahead of them
+    limit_of = [0, 7, dim - 1]
+    others = np.setdiff1d(np.arange(dim), limit_of)
+    shape = lambda x: x.reshape(len(x), -1, dim)  # noqa: E731
+    for columns, many in ((others, None), (limit_of, 97)):
+        for a, c, n in zip(q_starts, k_starts, new):
+            m = n if many is None else many
+            i, j = np.arange(m)[:, None], np.arange(m + behind)[None, :]
+            want, size = plain.attention(shape(vq)[a:a + m], shape(vk)[c:c + m + behind], shape(finite)[c:c + m + behind], dim ** -0.5, j <= i + behind)
+            terms = np.abs(shape(vq)[a:a + m]).sum(-1).max() * np.abs(vk[c:c + m + behind]).max() * dim ** -0.5
+            limit = plain.EPS[dtype] / 2 * (2 * np.abs(want) + size) * 1.01 + (terms * 2.0 ** -20 + 2.0 ** -18) * size + 1e-30
+            assert (np.abs(got[a:a + m] - want) <= limit)[:, :, columns].all(), (a, n, dim, columns[:3])
