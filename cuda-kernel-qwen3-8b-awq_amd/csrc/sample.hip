@@ -374,9 +374,9 @@ struct Choose {
       if (order >= a && order < b) f(order);
     }
   }
-  // the chunks of bin j's n tokens, and the tokens themselves where they are few; a, b: their orders
+  // the chunks of bin j's n tokens (bin kBins: of those beyond the bins), and the tokens themselves where they are few; a, b: their orders
   __device__ __forceinline__ void gather(int j, int n, uint64_t& a, uint64_t& b) const {
-    const uint32_t low = lowest_key(j);
+    const uint32_t low = j < kBins ? lowest_key(j) : key_of(-INFINITY) + 1;
     a = (uint64_t)low << 32;
     b = (uint64_t)(j ? lowest_key(j - 1) : key_of(largest) + 1) << 32;
     __syncthreads();  // the last bin's readers are done
@@ -523,8 +523,10 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
   __syncthreads();
   const uint64_t* const histogram = s.histogram + row * S * kBins;
 
+  // A uniform number this close to 0 asks for the first tokens, whose weights may be those that the sums do without.
+  const bool least = !(uniform_number >= 0x1p-60f);
   int end = kBins;          // bins below it are kept whole, those above it not at all
-  uint64_t border = 0;      // of bin `end` the tokens that are not behind this in order
+  uint64_t border = 0;      // of bin `end` the tokens that are not behind this in order (of those beyond the bins where it is kBins)
   float lightest = -INFINITY;  // no token behind this logit is kept
   bool at_least = false;    // and those of them that weigh at least min_p
   const double heaviest = uniform((double)largest * r.per_t * 0.125);
@@ -570,6 +572,7 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
       return Found<double>{64 * many + from, uniform(__shfl(ahead, from, 64)), base_count + uniform((uint32_t)__shfl((int)(count_upto - count), from, 64))};
     };
     double all = last_lane(many_upto);
+    const uint32_t in_bins = (uint32_t)__builtin_amdgcn_readlane((int)lanes::upto(count_of_many), 63);
     uint64_t from = 0, to = 0;  // the orders of bin `end`
     // top-k, top-p and min-p, each within what those ahead of it keep
 #pragma unroll 1
@@ -581,16 +584,19 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
         if (filter == 0 ? r.top_k == 0 : !(r.top_p < 1.0f)) continue;
         const double target = (double)r.top_p * all;
         Found<double> f = first_bin([&](double su, uint32_t n) { return filter ? su >= target : n >= (uint32_t)r.top_k; });
-        if (f.at == kBins) continue;
+        // fewer tokens within the bins than top-k keeps: sums do without the others, their order matters if the first tokens are asked for
+        if (f.at == kBins && (filter || !least)) continue;
         j = min(f.at, end);
         if (j < f.at) {  // (a rounding away from all that top-k keeps: the bin that it ends in)
           f.sum = 0.0;
           for (int i = 0; i < j; ++i) f.sum += (double)m.fixed[i] * kUnit * m.table[i];
           f.sum = uniform(f.sum);
         }
-        need = r.top_k - f.count;
-        reach = uniform((target - f.sum) / (kUnit * m.table[j]));
-        if (filter == 0) all = f.sum;  // and what is kept of bin j
+        need = r.top_k - (j < kBins ? f.count : in_bins);
+        if (j < kBins) {
+          reach = uniform((target - f.sum) / (kUnit * m.table[j]));
+          if (filter == 0) all = f.sum;  // and what is kept of bin j
+        }
       } else {
         if (!(r.min_p > 0.0f)) continue;
         const double d = top - floor((heaviest + log((double)r.min_p)) * 8.0);
@@ -600,12 +606,13 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
         if (j == end) continue;
         border = 0;
       }
-      const int n = uniform((int)m.bin_count[j]);
-      if (j != end) c.gather(j, n, from, to);
+      const int n = j < kBins ? uniform((int)m.bin_count[j]) : kHeld + 1;  // (those beyond the bins are not held)
+      if (j != end || j == kBins) c.gather(j, n, from, to);
       if (filter < 2) {
         c.last_kept(n, from, to, filter == 1, need, reach);
         const uint64_t last = uniform(m.word[0]);
         border = j == end && border > last ? border : last;
+        if (j == kBins) continue;
         if (filter == 0) all = uniform(all + (double)m.word[1] * kUnit * m.table[j]);
       }
       end = j;
@@ -653,16 +660,15 @@ __global__ __launch_bounds__(kChoose) void choose_kernel(SampleArgs s) {
   const Found<double> in_part = first_full(of_part, nothing, [&](double su, uint32_t) { return su > target; });
   double base = in_part.sum;
   int part = in_part.at < 64 ? in_part.at : 0;  // (a row has some weight, so one of its parts is it)
-  // A uniform number this close to 0 asks for the first tokens, whose weights may be those that the sums do without: part after part.
-  const bool least = target < total * 0x1p-60;
-  if (least) base = 0.0, part = 0;
+  if (least) base = 0.0, part = 0;  // part after part
   const auto weight_of_token = [&](T logit_of_it, int id) __attribute__((always_inline)) {
     const float l = c.of(logit_of_it);
     if (l < lightest) return 0.0;
     const Binned b = binned(l, r);
     const int j = c.below(b, l);
     if (j < end || (j == end && j < kBins && order_of(l, id) >= border && (!at_least || heavy(l)))) return weight_of(b) * m.table[j];
-    return least && j == kBins && end == kBins ? exp((double)l * r.per_t * 0.125 - heaviest) : 0.0;
+    const bool beyond = least && j == kBins && end == kBins && order_of(l, id) >= border && (!(r.min_p > 0.0f) || heavy(l));
+    return beyond ? exp((double)l * r.per_t * 0.125 - heaviest) : 0.0;
   };
   constexpr int kEach = kPart / kChoose;
   for (;; ++part) {

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import batch_plain as plain
-from test_gpu_batch import dev, packed, rng_of  # noqa: F401
+from test_gpu_batch import check_sample, dev, packed, rng_of, sample  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +48,31 @@ def test_packed_attention_beside_what_is_not_finite_in_a_step_that_some_wavefron
             terms = np.abs(shape(vq)[a:a + m]).sum(-1).max() * np.abs(vk[c:c + m + behind]).max() * dim ** -0.5
             limit = plain.EPS[dtype] / 2 * (2 * np.abs(want) + size) * 1.01 + (terms * 2.0 ** -20 + 2.0 ** -18) * size + 1e-30
             assert (np.abs(got[a:a + m] - want) <= limit)[:, :, columns].all(), (a, n, dim, columns[:3])
+
+
+# --- sampling -------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [5, 31, 5000, 8193, 40000])
+def test_sample_of_uniform_numbers_next_to_zero(dev, dtype, vocab):
+    """the first token kept, however little it weighs: also where fewer tokens than top-k keeps, or than weigh min-p, are within e^-64 of the largest"""
+    rng = rng_of("zero", dtype, vocab)
+    print("sample, zero", dtype, vocab, flush=True)
+    n = 12
+    x = rng.standard_normal((n, vocab))
+    x[0, vocab // 2:vocab // 2 + 10] += 90
+    x[1] = np.round(2 * x[1]) * 40              # many equals
+    x[2] = np.where(np.arange(vocab) % 3 == 1, 9.0, -1e4)
+    x[3] = -np.inf
+    x[3, [vocab // 3, vocab - 1]] = -100.0, 0.0
+    x[4, vocab // 2] = np.inf
+    x[5, : vocab // 2] = np.nan
+    x[6] *= 40
+    x[7, vocab // 4:] = -np.inf
+    d_x, vx = dev.act(x, dtype)
+    of = lambda *v: [v[i % len(v)] for i in range(n)]  # noqa: E731
+    k = of(50, 3, 2, 5, 1000, 4, 20, 4999, 1, 8190)
+    for u in (0.0, 1e-30, 2.0 ** -61, 2.0 ** -149):
+        for t, kk, p, m in ((of(1.0), k, None, None), (of(0.02, 0.05), k, None, None), (of(0.01), None, None, of(1e-30, 1e-35, 1e-28, 1e-27)), (of(0.02), k, None, of(1e-30, 0.0, 1e-37)),
+                            (of(0.02), k, of(1.0, 0.9, 0.999999), of(0.0, 1e-20)), (of(1e-3, 3e38, 1e-30), k, None, None), (of(0.02), None, None, None)):
+            us = np.full(n, u, np.float32)
+            check_sample(dev, dtype, vx, sample(dev, dtype, d_x, us, t, kk, p, m), us, t, kk, p, m)
