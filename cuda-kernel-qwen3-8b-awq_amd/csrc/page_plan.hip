@@ -80,11 +80,21 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(awq_page_plan_args a
     const Three at = sums_ahead(Three{back, 0, 0}, part, all);
     sums[tid] = at.a;
     __syncthreads();
-    for (int t = tid; t < all.a; t += kPlanThreads) {
-      const int r = last_not_above(sums, kPlanThreads, t);  // (of requests that begin at one sum the last is the one with pages)
-      if (available + t < a.n_pages) a.free_pages[available + t] = a.table[(int64_t)(i0 + r) * a.max_pages + t - sums[r]];
+    for (int t0 = 0; t0 < all.a; t0 += kPlanThreads) {
+      const int t = t0 + tid;
+      int page = -1, to = available + tid, many = min(all.a - t0, kPlanThreads);
+      if (t < all.a) {
+        const int r = last_not_above(sums, kPlanThreads, t);  // (of requests that begin at one sum the last is the one with pages)
+        page = held_page(a.table[(int64_t)(i0 + r) * a.max_pages + t - sums[r]], a.n_pages);
+      }
+      if (__syncthreads_or(t < all.a && page < 0)) {  // an entry that is no page is passed over
+        Three pages_of_these;
+        to = available + sums_ahead(Three{page >= 0 ? 1 : 0, 0, 0}, part, pages_of_these).a;
+        many = pages_of_these.a;
+      }
+      if (page >= 0 && to < a.n_pages) a.free_pages[to] = page;
+      available = min(available + many, a.n_pages);
     }
-    available = min(available + all.a, a.n_pages);
     __syncthreads();
   }
   int taken = 0, left = 0;

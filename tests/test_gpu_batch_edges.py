@@ -3,9 +3,33 @@ import numpy as np
 import pytest
 
 import batch_plain as plain
-from test_gpu_batch import check_sample, dev, packed, rng_of, sample  # noqa: F401
+from test_gpu_batch import check_plan, check_sample, dev, packed, rng_of, run_plan, sample, tables  # noqa: F401
 
 pytestmark = pytest.mark.gpu
+
+
+# --- pages and slots ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("n,width", [(1, 3), (6, 9), (40, 70), (300, 20), (1500, 5)])
+@pytest.mark.parametrize("plenty", [True, False], ids=["plenty", "short"])
+def test_plan_of_ended_requests_with_entries_that_are_no_pages(dev, n, width, plenty):
+    """what is no page does not go on the list, and nobody is given it"""
+    rng = rng_of("holes", n, plenty)
+    cached = rng.integers(0, 64 * width + 1, n)
+    fresh = rng.choice([-1, -1, 0, 1, 70], n)
+    fresh[0] = -1
+    table, n_pages = tables(rng, n, [plain.pages(c) for c in cached], width, 3 if n == 1 else 5 * n)
+    spare = np.setdiff1d(np.arange(n_pages), table)[: None if plenty else 1].tolist()
+    holes = rng.random(table.shape) < 0.2
+    table[holes] = rng.choice([-1, n_pages, -2 ** 31, 2 ** 31 - 1], holes.sum())
+    if n == 1:
+        table[0, 0] = -1
+    print("plan, holes", n, width, plenty, flush=True)
+    ended = fresh < 0
+    back = [p for i in np.flatnonzero(ended) for p in table[i, :plain.pages(cached[i])] if 0 <= p < n_pages]
+    total = int(np.maximum(fresh, 0).sum())
+    for max_tokens in (total, total + 5000):  # one launch and two
+        want = plain.plan(np.where(ended, 0, cached), np.where(ended, 0, fresh), table, spare + back, n_pages, max_tokens)
+        check_plan(run_plan(dev, cached, fresh, table, spare, n_pages, max_tokens), want, len(spare))
 
 
 # --- attention of packed prompts ----------------------------------------------------------------------------------------------
