@@ -117,6 +117,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(awq_page_plan_args a
       a.lengths[i] = length;
       a.starts[i] = base.b + at.b;
       if (a.key_starts) a.key_starts[i] = base.c + ahead.a;
+      // (for slots_kernel: `lengths` may be `cached`)
+      if (!SLOTS && put && base.b + at.b < a.max_tokens) a.positions[base.b + at.b] = cached;
     }
     sums[tid] = at.a;
     held_of[tid] = held;
@@ -158,6 +160,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(awq_page_plan_args a
   }
 }
 
+// The first position of a request's new ones is there already, and is written again as it is.
 __global__ __launch_bounds__(kSlotThreads) void slots_kernel(awq_page_plan_args a) {
   __shared__ int starts[kSlotStarts];
   const int n = a.n_requests;
@@ -173,8 +176,8 @@ __global__ __launch_bounds__(kSlotThreads) void slots_kernel(awq_page_plan_args 
     a.slots[t] = -1;
     return;
   }
-  const int r = here ? last_not_above(starts, n, (int)t) : last_not_above(a.starts, n, (int)t);
-  write_slot(a, t, r, here ? starts[r] : a.starts[r], min(max(a.cached[r], 0), a.max_pages * kPage), a.lengths[r]);
+  const int r = here ? last_not_above(starts, n, (int)t) : last_not_above(a.starts, n, (int)t), start = here ? starts[r] : a.starts[r];
+  write_slot(a, t, r, start, a.positions[start], a.lengths[r]);
 }
 
 }  // namespace

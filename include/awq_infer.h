@@ -716,7 +716,7 @@ int64_t awq_page_bytes(int32_t kv_heads, int32_t dim);
  * left out; one that needs pages is left out too where all that the requests up to it need together is
  * more than there are.  A request left out keeps the positions it has, its new
  * ones get slot -1.  Written: table (new entries), free_pages, *free_out (may be
- * free_in), lengths [n] (positions that the requests have then; ended ones 0), starts [n + 1] and key_starts
+ * free_in), lengths [n] (positions that the requests have then; ended ones 0; may be cached), starts [n + 1] and key_starts
  * [n + 1] (sums of the fresh positions and of lengths ahead of each request; key_starts may be NULL), positions
  * and slots of max_tokens rows (of the fresh positions one request behind the
  * other; rows behind the last: position 0, slot -1), *left_out (requests left out, may be NULL). */

@@ -1,4 +1,6 @@
 """Several requests at once: what lies at the edges of the operators' definitions, against batch_plain.py's 64 bits."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -30,6 +32,33 @@ def test_plan_of_ended_requests_with_entries_that_are_no_pages(dev, n, width, pl
     for max_tokens in (total, total + 5000):  # one launch and two
         want = plain.plan(np.where(ended, 0, cached), np.where(ended, 0, fresh), table, spare + back, n_pages, max_tokens)
         check_plan(run_plan(dev, cached, fresh, table, spare, n_pages, max_tokens), want, len(spare))
+
+@pytest.mark.parametrize("n", [5, 300, 1500])
+@pytest.mark.parametrize("more", [0, 5000])
+def test_plan_with_the_lengths_in_the_place_of_those_before(dev, n, more):
+    """one buffer of lengths, step after step: in one launch and in two"""
+    rng = rng_of("in place", n, more)
+    width = 12
+    print("plan, in place", n, more, flush=True)
+    lengths = rng.integers(0, 64 * width - 100, n)
+    table, n_pages = tables(rng, n, [plain.pages(c) for c in lengths], width, 4 * n)
+    spare = np.setdiff1d(np.arange(n_pages), table).tolist()
+    d = {name: dev.ints(x) for name, x in (("table", table), ("free", spare + [-7] * (n_pages - len(spare))), ("count", [len(spare)]), ("lengths", lengths))}
+    for _ in range(3):
+        fresh = rng.choice([-1, 0, 1, 1, 65, 200], n)
+        total = int(np.maximum(fresh, 0).sum())
+        T = total + more
+        stack = dev.host(d["free"])[:int(dev.host(d["count"])[0])].tolist()
+        want = plain.plan(dev.host(d["lengths"]), fresh, dev.host(d["table"]), stack, n_pages, T)
+        d_fresh, starts, keys, positions, slots, left = dev.ints(fresh), *(dev.full((m,), -7, dev.torch.int32) for m in (n + 1, n + 1, T + 1, T + 1, 1))
+        a = dev.awq.AwqPagePlanArgs(d["lengths"].data_ptr(), d_fresh.data_ptr(), d["table"].data_ptr(), d["free"].data_ptr(), d["count"].data_ptr(),
+                                    d["count"].data_ptr(), d["lengths"].data_ptr(), starts.data_ptr(), keys.data_ptr(), positions.data_ptr(), slots.data_ptr(),
+                                    left.data_ptr(), T, n, width, n_pages, 0)
+        dev.awq.check(dev.lib.awq_page_plan(ctypes.byref(a), dev.stream()))
+        h = dev.host
+        assert h(d["lengths"]).tolist() == want[3] and h(starts).tolist() == want[4] and h(keys).tolist() == want[5] and int(h(left)[0]) == want[8]
+        assert np.array_equal(h(d["table"]), want[0]) and int(h(d["count"])[0]) == want[2]
+        assert h(positions)[:T].tolist() == want[6] and h(slots)[:T].tolist() == want[7] and h(positions)[T] == h(slots)[T] == -7
 
 
 # --- attention of packed prompts ----------------------------------------------------------------------------------------------
