@@ -11,6 +11,7 @@ typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;     // of a workgroup, each with pages of its own
 constexpr int kColumns = 16;  // query heads of one key/value head that share a pass over the pages
+constexpr float kSlack = 8.0f;
 
 // Wavefronts of a SIMD: as many as have all their numbers in registers.  Heads of 128, 64 requests of 8 key/value heads with 4 query heads each:
 // 4 (some numbers in scratch memory) 49 us, 3 42, 2 44; 2 key/value heads with 16: 4 37 us, 2 20; heads of 256 with 16: 2 39 us, 1 25.
@@ -81,8 +82,9 @@ __device__ __forceinline__ int run_of(int all, int workers) { return (all + work
 // sum over a group, s sum(q n) + z sum(q) in binary32, and on the weights, p s rounded to binary16 for the product, p z in binary32.
 // Heads of 128, 32 over 8: 64 requests of 100 to 8,000 positions, bfloat16, 42 us, 4.2 TB/s of the cache; one of 40,960 positions, binary16, 17 us (its
 // 640 pages leave a worker two); 12 requests of 5 to 300 positions, 16 heads of 64, 6 us.  Bound by memory and, at a few pages a worker, by the start.
-// Weights are relative to the largest of score + exponent of the page's largest value scale, so that p s is below 1 and as exact as
-// binary16 can be whatever the values' size.
+// Weights are relative to the largest score, rounded up to a whole number so that moving it is exact.  A group's products p s are relative to a power of
+// two of its own, 2^r times that, which moves once some are 2^kSlack above it: they are normal numbers of binary16 down to 2^-14 of the group's largest
+// so far, whatever the scales of keys that weigh nothing and of other groups, and whatever their sign.
 template <typename T, int D, int COLUMNS>
 __global__ __launch_bounds__(64 * kWaves, resident(D, COLUMNS)) void paged_kernel(PagedArgs p) {
   constexpr int G = D / 64, PIECES = D / 32;  // groups; 16-byte pieces of a row
@@ -231,10 +233,11 @@ __global__ __launch_bounds__(64 * kWaves, resident(D, COLUMNS)) void paged_kerne
     }
 
     f32x4_t o[G][4];
-    float off[G], best = -INFINITY, sum = 0.0f;
+    float off[G], r2[G], best = -INFINITY, sum = 0.0f;  // r2: the group's r
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       off[g] = 0.0f;
+      r2[g] = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[g][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -296,7 +299,6 @@ __global__ __launch_bounds__(64 * kWaves, resident(D, COLUMNS)) void paged_kerne
         }
       }
       half4_t vs[SETS][G], vz[SETS][G];
-      half4_t widest4 = half4_t{};
 #pragma unroll
       for (int q = 0; q < SETS; ++q) {
         const int row = 16 * (q * TP + mine) + 4 * kg;
@@ -312,42 +314,56 @@ __global__ __launch_bounds__(64 * kWaves, resident(D, COLUMNS)) void paged_kerne
             for (int e = 0; e < 4; ++e)
               if (row + e >= left) vs[q][g][e] = vz[q][g][e] = (half_t)0.0f;
         }
-#pragma unroll
-        for (int g = 0; g < G; ++g) widest4 = __builtin_elementwise_max(widest4, vs[q][g]);
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the keys and the parameters have been read
       if (next >= 0) request_keys(next);
       highest = over_head<COLUMNS>(highest, lanes::Max());
-      const float widest = over_head<COLUMNS>(fmaxf(fmaxf((float)widest4[0], (float)widest4[1]), fmaxf((float)widest4[2], (float)widest4[3])), lanes::Max());
-      const float to_best = fmaxf(best, highest + (float)(widest > 0.0f ? __builtin_amdgcn_frexp_expf(widest) : -24));
+      const float to_best = fmaxf(best, __builtin_ceilf(highest));
       if (__builtin_amdgcn_ballot_w64(to_best > best)) {
-        const float alpha = to_best > best ? __builtin_amdgcn_exp2f(best - to_best) : 1.0f;
+        const float step = to_best > best ? to_best - best : 0.0f, alpha = __builtin_amdgcn_exp2f(-step);
         best = to_best;
         sum *= alpha;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           off[g] *= alpha;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[g][j] *= alpha;
+          r2[g] -= step;  // (the sums of products stay as they are)
         }
       }
       const float base = best == -INFINITY ? 0.0f : best;
-      u32x2_t weights[SETS][G];  // times the scales, four in binary16
+      float w[SETS][4];
 #pragma unroll
-      for (int q = 0; q < SETS; ++q) {
-        half4_t ps[G];
+      for (int q = 0; q < SETS; ++q)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float w = __builtin_amdgcn_exp2f(score[q][e] - base);
-          sum += w;
-#pragma unroll
-          for (int g = 0; g < G; ++g) {
-            ps[g][e] = (half_t)(w * (float)vs[q][g][e]);
-            off[g] = __builtin_fmaf(w, (float)vz[q][g][e], off[g]);
-          }
+          w[q][e] = __builtin_amdgcn_exp2f(score[q][e] - base);
+          sum += w[q][e];
         }
+      u32x2_t weights[SETS][G];  // times the scales, four in binary16
 #pragma unroll
-        for (int g = 0; g < G; ++g) weights[q][g] = __builtin_bit_cast(u32x2_t, ps[g]);
+      for (int g = 0; g < G; ++g) {
+        float widest = 0.0f;
+#pragma unroll
+        for (int q = 0; q < SETS; ++q)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            widest = fmaxf(widest, fabsf(w[q][e] * (float)vs[q][g][e]));
+            off[g] = __builtin_fmaf(w[q][e], (float)vz[q][g][e], off[g]);
+          }
+        if (__builtin_amdgcn_ballot_w64(widest > __builtin_amdgcn_exp2f(r2[g] + kSlack))) {
+          const float all = over_head<COLUMNS>(widest, lanes::Max()), to = all > 0.0f ? fmaxf((float)__builtin_amdgcn_frexp_expf(all), r2[g]) : r2[g];
+          const float alpha = to > r2[g] ? __builtin_amdgcn_exp2f(r2[g] - to) : 1.0f;
+          r2[g] = to;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[g][j] *= alpha;
+        }
+        const float up = __builtin_amdgcn_exp2f(fminf(-r2[g], 126.0f));
+#pragma unroll
+        for (int q = 0; q < SETS; ++q) {
+          half4_t ps;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ps[e] = (half_t)(w[q][e] * (float)vs[q][g][e] * up);
+          weights[q][g] = __builtin_bit_cast(u32x2_t, ps);
+        }
       }
       if (next >= 0) wait_for_requests<kKeyLoads>();
       else wait_for_requests<0>();
@@ -409,10 +425,11 @@ __global__ __launch_bounds__(64 * kWaves, resident(D, COLUMNS)) void paged_kerne
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       off[g] = over_head<COLUMNS>(off[g], lanes::Add());
+      const float size = __builtin_amdgcn_exp2f(r2[g]);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[g][j][e] = __builtin_fmaf(add_columns(o[g][j][e]), j % 2 ? 0x1p20f : 0x1p24f, off[g]);
+        for (int e = 0; e < 4; ++e) o[g][j][e] = __builtin_fmaf(add_columns(o[g][j][e]) * size, j % 2 ? 0x1p20f : 0x1p24f, off[g]);
     }
     // o[g][j][e]: value 64 g + 16 kg + 4 e + j of the lane's head
     bool whole = from == 0 && to == n_pages, writes = m < columns;
@@ -473,7 +490,9 @@ __global__ __launch_bounds__(64 * kWaves, resident(D, COLUMNS)) void paged_kerne
     } else if (writes) {
       // (a worker has two such requests at most: the one that its run begins in and the one that it ends in)
       const int64_t slot = ((int64_t)stream * p.workers + worker) * 2 + (start < begin ? 0 : 1);
-      float* const out = p.sums + (slot * p.columns + m) * D + 16 * kg;
+      int quarter = kg;
+      if constexpr (D == 256) asm volatile("" : "+v"(quarter));  // (formed anew: an address that waits through the pages would be one number too many)
+      float* const out = p.sums + (slot * p.columns + m) * D + 16 * quarter;
 #pragma unroll
       for (int g = 0; g < G; ++g)
 #pragma unroll

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import batch_plain as plain
-from test_gpu_batch import check_plan, check_sample, dev, packed, rng_of, run_plan, sample, tables  # noqa: F401
+from test_gpu_batch import check_paged, check_plan, check_sample, dev, packed, paged, rng_of, run_plan, sample, tables  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -59,6 +59,57 @@ def test_plan_with_the_lengths_in_the_place_of_those_before(dev, n, more):
         assert h(d["lengths"]).tolist() == want[3] and h(starts).tolist() == want[4] and h(keys).tolist() == want[5] and int(h(left)[0]) == want[8]
         assert np.array_equal(h(d["table"]), want[0]) and int(h(d["count"])[0]) == want[2]
         assert h(positions)[:T].tolist() == want[6] and h(slots)[:T].tolist() == want[7] and h(positions)[T] == h(slots)[T] == -7
+
+
+# --- attention over pages ---------------------------------------------------------------------------------------------------
+def cache_of_scales(dev, rng, n_pages, kv, dim, v_scales, k_signs=False):
+    """a random cache with values of these scales [pages][heads][64][dim / 64]: (tensor, keys, values, the size of the values' parts)"""
+    shape = (n_pages, kv, 64, dim)
+    n = [rng.integers(0, 16, shape).astype(np.float64) for _ in range(2)]
+    s = [plain.nearest(x, "f16") for x in (0.2 * (rng.choice([-1.0, 1.0], v_scales.shape) if k_signs else np.ones(v_scales.shape)), v_scales)]
+    z = [plain.nearest(x * (-7.5 + rng.standard_normal(x.shape)), "f16") for x in s]
+    cache = dev.torch.from_numpy(plain.packed_pages(*zip(n, s, z))).cuda()
+    return cache, plain.value_of(n[0], s[0], z[0]), plain.value_of(n[1], s[1], z[1]), plain.value_of(n[1], np.abs(s[1]), np.abs(z[1]))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (12, 2, 128), (16, 1, 128), (8, 2, 256), (16, 1, 256)])
+@pytest.mark.parametrize("gain", [0.3, 6.0])
+@pytest.mark.parametrize("kind", ["keys", "groups", "both", "pages", "none"])
+def test_paged_attention_of_scales_far_apart(dev, dtype, heads, kv, dim, gain, kind):
+    """scales of values that differ by up to 2^20 between keys, between groups, between both or from page to page, and groups without any: the tolerance is
+    that of even ones, which counts what each key weighs"""
+    lengths = [700, 1300, 64, 3]
+    rng = rng_of("far", dtype, heads, dim, gain * 10, kind)
+    print("paged, scales", dtype, heads, kv, dim, gain, kind, flush=True)
+    table, n_pages = tables(rng, 4, [plain.pages(x) for x in lengths], 21)
+    shape = (n_pages, kv, 64, dim // 64)
+    cut = {"keys": (n_pages, kv, 64, 1), "groups": (1, kv, 1, dim // 64), "both": shape, "pages": (n_pages, 1, 1, 1), "none": (n_pages, kv, 64, 1)}[kind]
+    scales = np.broadcast_to(2.0 ** rng.uniform(-12, 8, cut), shape).copy()
+    if kind == "none":
+        scales[..., 0] = 0.0
+        scales[:, :, 5:9] = 0.0
+    cache, k, v, spread = cache_of_scales(dev, rng, n_pages, kv, dim, scales)
+    d_q, vq = dev.act(rng.standard_normal((4, heads * dim)) * gain, dtype)
+    got = paged(dev, dtype, d_q, cache, table, lengths, heads, kv, dim, dim ** -0.5, dev.full((4, heads * dim), 9.0, dtype))
+    check_paged(got.reshape(4, heads, dim), dtype, vq.reshape(4, heads, dim), table, lengths, k, v, spread, n_pages, dim ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (12, 2, 128), (16, 1, 256)])
+@pytest.mark.parametrize("size", [1e-4, 1.0, 500.0])
+@pytest.mark.parametrize("mixed", [True, False], ids=["mixed", "negative"])
+def test_paged_attention_of_scales_below_zero(dev, dtype, heads, kv, dim, size, mixed):
+    lengths = [700, 64, 129]
+    rng = rng_of("below", dtype, heads, dim, size * 1e4, mixed)
+    print("paged, below zero", dtype, heads, kv, dim, size, mixed, flush=True)
+    table, n_pages = tables(rng, 3, [plain.pages(x) for x in lengths], 11)
+    shape = (n_pages, kv, 64, dim // 64)
+    scales = size * np.exp(0.5 * rng.standard_normal(shape)) * (rng.choice([-1.0, 1.0], shape) if mixed else -1.0)
+    cache, k, v, spread = cache_of_scales(dev, rng, n_pages, kv, dim, scales, k_signs=True)
+    d_q, vq = dev.act(rng.standard_normal((3, heads * dim)), dtype)
+    got = paged(dev, dtype, d_q, cache, table, lengths, heads, kv, dim, dim ** -0.5, dev.full((3, heads * dim), 9.0, dtype))
+    check_paged(got.reshape(3, heads, dim), dtype, vq.reshape(3, heads, dim), table, lengths, k, v, spread, n_pages, dim ** -0.5)
 
 
 # --- attention of packed prompts ----------------------------------------------------------------------------------------------
