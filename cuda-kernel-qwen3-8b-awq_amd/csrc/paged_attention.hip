@@ -469,7 +469,7 @@ __global__ __launch_bounds__(64 * kWaves, resident(D, COLUMNS)) void paged_kerne
           const float inv = total != 0.0f ? 1.0f / total : 0.0f;
           typedef T four_t __attribute__((ext_vector_type(4)));
           *reinterpret_cast<four_t*>((T*)a.ctx + (int64_t)r * a.ldc + (int64_t)(head0 + c) * D + d) =
-              four_t{(T)(y[0] * inv), (T)(y[1] * inv), (T)(y[2] * inv), (T)(y[3] * inv)};
+              four_t{held(y[0] * inv, T()), held(y[1] * inv, T()), held(y[2] * inv, T()), held(y[3] * inv, T())};
         } else {
           *reinterpret_cast<f32x4_t*>(p.sums + (slot * p.columns + c) * D + d) = y;
           if (d == 0) p.ml[(slot * p.columns + c) * 2] = top, p.ml[(slot * p.columns + c) * 2 + 1] = total;
@@ -477,22 +477,22 @@ __global__ __launch_bounds__(64 * kWaves, resident(D, COLUMNS)) void paged_kerne
       }
       return;
     }
+    int quarter = kg, of_column = m;
+    if constexpr (D == 256) asm volatile("" : "+v"(quarter), "+v"(of_column));  // (addresses are formed anew: one that waits through the pages would be a number too many)
     if (whole && writes) {
       const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-      T* const out = (T*)a.ctx + (int64_t)r * a.ldc + (int64_t)(head0 + m) * D + 16 * kg;
+      T* const out = (T*)a.ctx + (int64_t)r * a.ldc + (int64_t)(head0 + of_column) * D + 16 * quarter;
       typedef T four_t __attribute__((ext_vector_type(4)));
 #pragma unroll
       for (int g = 0; g < G; ++g)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           *reinterpret_cast<four_t*>(out + 64 * g + 4 * e) =
-              four_t{(T)(o[g][0][e] * inv), (T)(o[g][1][e] * inv), (T)(o[g][2][e] * inv), (T)(o[g][3][e] * inv)};
+              four_t{held(o[g][0][e] * inv, T()), held(o[g][1][e] * inv, T()), held(o[g][2][e] * inv, T()), held(o[g][3][e] * inv, T())};
     } else if (writes) {
       // (a worker has two such requests at most: the one that its run begins in and the one that it ends in)
       const int64_t slot = ((int64_t)stream * p.workers + worker) * 2 + (start < begin ? 0 : 1);
-      int quarter = kg;
-      if constexpr (D == 256) asm volatile("" : "+v"(quarter));  // (formed anew: an address that waits through the pages would be one number too many)
-      float* const out = p.sums + (slot * p.columns + m) * D + 16 * quarter;
+      float* const out = p.sums + (slot * p.columns + of_column) * D + 16 * quarter;
 #pragma unroll
       for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -577,7 +577,7 @@ __global__ __launch_bounds__(kJoin) void paged_join_kernel(PagedArgs p, int chun
   if (share || value >= columns * D) return;
   for (int i = 1; i < min(shares, parts); ++i) add(best_of[i * quads + tid], sum_of[i * quads + tid], o_of[i * quads + tid]);
   const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-  *reinterpret_cast<four_t*>(out) = four_t{(T)(o[0] * inv), (T)(o[1] * inv), (T)(o[2] * inv), (T)(o[3] * inv)};
+  *reinterpret_cast<four_t*>(out) = four_t{held(o[0] * inv, T()), held(o[1] * inv, T()), held(o[2] * inv, T()), held(o[3] * inv, T())};
 }
 
 template <typename T, int D>

@@ -212,6 +212,13 @@ __global__ __launch_bounds__(256) void rows_kernel(awq_paged_rows_args a) {
     const half_t z = *reinterpret_cast<const half_t*>(base + page_parameter(dim, value, g, 1, in_page));
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = value_of((float)((word >> (4 * i)) & 15u), s, z, T());
+    if constexpr (__is_same(T, half_t)) {
+      const float furthest = fabsf(15.0f * (float)s + (float)z);  // (z is one of its numbers)
+      if (furthest > kHalfMax && furthest < INFINITY) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = (half_t)__builtin_amdgcn_fmed3f((float)y[i], -kHalfMax, kHalfMax);
+      }
+    }
   }
   T* const out = value ? (T*)a.v + row * a.ldv : (T*)a.k + row * a.ldk;
   *reinterpret_cast<eight_t*>(out + (int64_t)head * dim + at) = y;

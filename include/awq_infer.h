@@ -696,7 +696,8 @@ int awq_polynorm(void* z, int64_t ld, int64_t n, int64_t n_tokens, const float* 
  * dim 64, 128 or 256, 16-byte aligned.  A head's part of a page: its keys [64][dim / 2 bytes], its values
  * likewise, nibbles with the low one first; then the keys' parameters
  * [dim / 64][scale, offset][64] in binary16, then the values'.  64 values of a
- * position share a scale s and an offset z; nibble n stands for s n + z.  Nibble
+ * position share a scale s and an offset z; nibble n stands for s n + z; rows and contexts in binary16 that would be beyond
+ * its range (the fifteenth step of a group that spans it may be) are its largest number.  Nibble
  * k dim / 4 + 16 g + e of a key's row is its value 64 g + 16 k + e (k < 4, e < 16),
  * nibble c dim / 16 + 4 g + e of a value's row its value 64 g + 4 c + e (c < 16, e < 4).
  * `table` [n_requests][max_pages] names the page of every 64 positions of a

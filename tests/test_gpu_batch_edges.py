@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import batch_plain as plain
-from test_gpu_batch import check_paged, check_plan, check_sample, dev, packed, paged, rng_of, run_plan, sample, tables  # noqa: F401
+from test_gpu_batch import append, cache_of, check_paged, check_plan, check_sample, dev, packed, paged, rng_of, rows_of, run_plan, sample, tables  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -59,6 +59,47 @@ def test_plan_with_the_lengths_in_the_place_of_those_before(dev, n, more):
         assert h(d["lengths"]).tolist() == want[3] and h(starts).tolist() == want[4] and h(keys).tolist() == want[5] and int(h(left)[0]) == want[8]
         assert np.array_equal(h(d["table"]), want[0]) and int(h(d["count"])[0]) == want[2]
         assert h(positions)[:T].tolist() == want[6] and h(slots)[:T].tolist() == want[7] and h(positions)[T] == h(slots)[T] == -7
+
+
+# --- append and rows ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("written", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_values_at_the_end_of_binary16_stay_finite(dev, written, dim):
+    """groups that span all of binary16, whose fifteenth step lies beyond it: its largest number, for the rows and for the attention"""
+    kv, T = 2, 20
+    rng = rng_of("end", written, dim)
+    x = rng.choice([-65504.0, 65504.0, 0.0, 3.0], (T, kv * dim))
+    x[:4, 0], x[:4, 1] = -65504.0, 65504.0
+    x[4] = 65504.0
+    x[5], x[5, ::64] = -65504.0, 65504.0
+    x[6, ::64] = np.nan
+    if written == "bf16":
+        x[7] = rng.choice([-1e30, 1e30], kv * dim)
+    d_x, vx = dev.act(x, written)
+    cache = dev.torch.zeros((1, kv, 72 * dim), dtype=dev.torch.uint8, device="cuda")
+    append(dev, written, None, d_x, d_x, None, None, dev.ints(range(T)), dev.ints(range(T)), cache, 1, kv, dim, 0, False, None, None)
+    with np.errstate(invalid="ignore"):
+        values = plain.value_of(*plain.quantised(vx.reshape(T, kv, dim)))
+    assert np.abs(values[[0, 1, 2, 3, 5]]).max() > 65520.0
+    for dtype in ("f16", "bf16"):
+        want = plain.nearest(np.clip(values, -65504.0, 65504.0) if dtype == "f16" else values, dtype).reshape(T, -1)
+        for g in rows_of(dev, dtype, cache, np.array([[0]]), None, [T], [0, T], T, kv, dim, pad=0):
+            assert np.array_equal(np.isnan(g), np.isnan(want)) and np.array_equal(g[~np.isnan(g)], want[~np.isnan(want)])
+    # one position a request is the attention's result as it is; 3 requests, and one after the other
+    order = [0, 3, 5]
+    pages = dev.torch.cat([cache[:, :, :]] * T)
+    for i in range(T):  # position i first in page i
+        data, par = (t[i].view(kv, -1, 64, w) for t, w in ((pages[:, :, :64 * dim], dim // 2), (pages[:, :, 64 * dim:], 2)))
+        first = data[:, :, i].clone(), par[:, :, i].clone()
+        pages[i, :, :64 * dim].view(kv, 2, 64, dim // 2)[:, :, 0] = first[0]
+        pages[i, :, 64 * dim:].view(kv, -1, 64, 2)[:, :, 0] = first[1]
+    d_q, _ = dev.act(np.zeros((3, kv * dim)), "f16")
+    got = paged(dev, "f16", d_q, pages, np.array(order)[:, None], [1, 1, 1], kv, kv, dim, 0.1, dev.full((3, kv * dim), 9.0, "f16"))
+    want = np.clip(values[order], -65504.0, 65504.0).reshape(3, -1)
+    size = np.abs(values[order]).reshape(3, -1)
+    assert np.isfinite(got).all()
+    # a value's product and offset are rounded to 2^-11 of them, the result once more
+    assert (np.abs(got - want) <= 2.0 ** -11 * (np.abs(want) + 131008.0 + size)).all()
 
 
 # --- attention over pages ---------------------------------------------------------------------------------------------------
