@@ -21,8 +21,8 @@ __host__ __device__ inline int page_parameter(int dim, int value, int g, int whi
 __host__ __device__ inline int held_page(int entry, int n_pages) { return entry >= 0 && entry < n_pages ? entry : -1; }
 __host__ __device__ inline int slot_page(int slot, int n_pages) { return slot >= 0 && slot / kPage < n_pages ? slot / kPage : -1; }
 
-// A page's values and their means (of finite scales and offsets) as the activations' type has them: 15 s + z may lie beyond binary16's, whose
-// largest it is then.
+// Means of values as the activations' type has them: what is finite and beyond binary16 is its largest number (15 s + z may be, and the mean of
+// values at its end under rounded weights).
 __device__ __forceinline__ half_t held(float v, half_t) { return (half_t)(fabsf(v) < INFINITY ? __builtin_amdgcn_fmed3f(v, -65504.0f, 65504.0f) : v); }
 __device__ __forceinline__ bf16_t held(float v, bf16_t) { return (bf16_t)v; }
 

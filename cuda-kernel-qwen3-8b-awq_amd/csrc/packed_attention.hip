@@ -366,7 +366,7 @@ __global__ __launch_bounds__(256, WAVES) void packed_kernel(awq_packed_attention
     for (int u = 0; u < 4; ++u) {
       four_t v;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = (T)(o[d][4 * u + j] * inv);
+      for (int j = 0; j < 4; ++j) v[j] = held(o[d][4 * u + j] * inv, T());  // (rounded weights may lead a little beyond the largest value)
       *reinterpret_cast<four_t*>(out + 32 * d + 8 * u + 4 * kh) = v;
     }
 }

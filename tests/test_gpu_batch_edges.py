@@ -195,6 +195,20 @@ def test_packed_attention_beside_what_is_not_finite_in_a_step_that_some_wavefron
             assert (np.abs(got[a:a + m] - want) <= limit)[:, :, columns].all(), (a, n, dim, columns[:3])
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("score", [0.716796875, 1.3984375, 3.494140625])
+def test_packed_attention_of_values_at_the_end_of_binary16(dev, dim, score):
+    """weights e^score that binary16 rounds up by some 4.5e-4, of values that are its largest number: their mean is that number"""
+    n, q = 2048, np.zeros((5, dim))
+    q[:, 0] = 1.0
+    k, v = np.zeros((n, dim)), np.full((n, dim), 65504.0)
+    k[64:, 0] = score
+    v[:, 1::2] *= -1.0
+    (d_q, _), (d_k, _), (d_v, vv) = (dev.act(x, "f16") for x in (q, k, v))
+    got = packed(dev, "f16", d_q, d_k, d_v, [0, 5], [0, n], 1, 1, dim, False, 1.0, dev.full((5, dim), 9.0, "f16"))
+    assert np.isfinite(got).all() and (np.abs(got - vv[:5]) <= 2.0 ** -10 * 65504.0).all()
+
+
 # --- sampling -------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("vocab", [5, 31, 5000, 8193, 40000])
