@@ -26,6 +26,8 @@ __host__ __device__ inline int slot_page(int slot, int n_pages) { return slot >=
 __device__ __forceinline__ half_t held(float v, half_t) { return (half_t)(fabsf(v) < INFINITY ? __builtin_amdgcn_fmed3f(v, -65504.0f, 65504.0f) : v); }
 __device__ __forceinline__ bf16_t held(float v, bf16_t) { return (bf16_t)v; }
 
+inline bool launchable(int64_t blocks, int threads) { return blocks * threads < (1ll << 32); }  // HIP takes no more
+
 int launch_page_plan(const awq_page_plan_args& a, hipStream_t st);
 int launch_paged_append(const awq_paged_append_args& a, bool bf16, hipStream_t st);
 int launch_paged_rows(const awq_paged_rows_args& a, bool bf16, hipStream_t st);

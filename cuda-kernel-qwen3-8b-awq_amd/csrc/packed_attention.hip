@@ -374,7 +374,7 @@ __global__ __launch_bounds__(256, WAVES) void packed_kernel(awq_packed_attention
 template <typename T>
 int launch(const awq_packed_attention_args& a, hipStream_t st) {
   const int64_t tiles = a.n_tokens / kQueries + std::min<int64_t>(a.n_requests, a.n_tokens);
-  AWQ_REQUIRE(tiles * a.heads < (1ll << 31), "too many queries and heads");
+  AWQ_REQUIRE(launchable(tiles * a.heads, 256), "too many queries and heads");
   const dim3 grid((unsigned)(tiles * a.heads));
   if (a.dim == 64) hipLaunchKernelGGL((packed_kernel<T, 64, 64, 2>), grid, dim3(256), 0, st, a);
   else if (a.dim == 128) hipLaunchKernelGGL((packed_kernel<T, 128, 64, 2>), grid, dim3(256), 0, st, a);

@@ -587,6 +587,11 @@ void launch_pages(const PagedArgs& p, dim3 grid, hipStream_t st) {
   else hipLaunchKernelGGL((paged_kernel<T, D, 16>), grid, dim3(64 * kWaves), 0, st, p);
 }
 
+// wide pieces of a request's values where the workers are cut over many requests, few parts each; narrow ones, whose threads share the parts,
+// where they are cut over few (one request of 40,960 positions 5.5 us with 32 pieces, 7.2 with 128; 64 requests 17.8 and 9.2)
+int quads_of(const PagedArgs& p) { return p.workers / kWaves > 16ll * p.a.n_requests ? 32 : 128; }
+int chunks_of(const PagedArgs& p) { return (p.columns * p.a.dim + 4 * quads_of(p) - 1) / (4 * quads_of(p)); }
+
 template <typename T>
 int launch(const PagedArgs& p, hipStream_t st) {
   const dim3 grid((unsigned)(p.workers / kWaves * p.streams));
@@ -594,10 +599,7 @@ int launch(const PagedArgs& p, hipStream_t st) {
   else if (p.a.dim == 128) launch_pages<T, 128>(p, grid, st);
   else launch_pages<T, 256>(p, grid, st);
   AWQ_HIP_TRY(hipGetLastError());
-  // wide pieces of a request's values where the workers are cut over many requests, few parts each; narrow ones, whose threads share the parts,
-  // where they are cut over few (one request of 40,960 positions 5.5 us with 32 pieces, 7.2 with 128; 64 requests 17.8 and 9.2)
-  const int quads = p.workers / kWaves > 16 * p.a.n_requests ? 32 : 128;
-  const int chunks = (p.columns * p.a.dim + 4 * quads - 1) / (4 * quads);
+  const int quads = quads_of(p), chunks = chunks_of(p);
   hipLaunchKernelGGL(paged_join_kernel<T>, dim3((unsigned)(p.a.n_requests * p.streams * chunks)), dim3(kJoin), 0, st, p, chunks, quads);
   AWQ_HIP_TRY(hipGetLastError());
   return AWQ_OK;
@@ -618,6 +620,7 @@ int launch_paged_attention(const awq_paged_attention_args& u, bool bf16, hipStre
   p.columns = columns_of(u.heads / u.kv_heads);
   p.sums = (float*)u.workspace;
   p.ml = p.sums + (int64_t)p.streams * p.workers * 2 * p.columns * u.dim;
-  AWQ_REQUIRE((int64_t)u.n_requests * p.streams * p.columns * u.dim / 64 < (1ll << 31), "too many requests and heads");
+  AWQ_REQUIRE(launchable((int64_t)p.workers / kWaves * p.streams, 64 * kWaves) && launchable((int64_t)u.n_requests * p.streams * chunks_of(p), kJoin),
+              "too many requests and heads");
   return bf16 ? launch<bf16_t>(p, st) : launch<half_t>(p, st);
 }

@@ -230,7 +230,7 @@ int launch_paged_append(const awq_paged_append_args& a, bool bf16, hipStream_t s
   const int items = (a.q ? a.heads : 0) + (a.k ? a.kv_heads : 0) + (a.k && a.cache ? a.kv_heads : 0);
   if (a.n_tokens == 0 || items == 0) return AWQ_OK;
   const int blocks = (items * (a.dim / 8) + 255) / 256;
-  AWQ_REQUIRE(a.n_tokens * blocks < (1ll << 31), "too many tokens and heads");
+  AWQ_REQUIRE(launchable(a.n_tokens * blocks, 256), "too many tokens and heads");
   const auto kernel = bf16 ? append_kernel<bf16_t> : append_kernel<half_t>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(a.n_tokens * blocks)), dim3(256), 0, st, a, blocks);
   AWQ_HIP_TRY(hipGetLastError());
@@ -240,7 +240,7 @@ int launch_paged_append(const awq_paged_append_args& a, bool bf16, hipStream_t s
 int launch_paged_rows(const awq_paged_rows_args& a, bool bf16, hipStream_t st) {
   if (a.n_rows == 0 || (!a.k && !a.v)) return AWQ_OK;
   const int64_t units = a.n_rows * ((a.k != nullptr) + (a.v != nullptr)) * (a.kv_heads * a.dim / 8);
-  AWQ_REQUIRE((units + 255) / 256 < (1ll << 31), "too many rows and heads");
+  AWQ_REQUIRE(launchable((units + 255) / 256, 256), "too many rows and heads");
   const auto kernel = bf16 ? rows_kernel<bf16_t> : rows_kernel<half_t>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)((units + 255) / 256)), dim3(256), 0, st, a);
   AWQ_HIP_TRY(hipGetLastError());

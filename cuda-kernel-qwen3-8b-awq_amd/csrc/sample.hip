@@ -744,7 +744,7 @@ int launch_sample(const awq_sample_args& a, int dtype, hipStream_t st) {
   s.a = a;
   s.parts = parts_of(a.vocab);
   s.chunks = chunks_of(a.vocab);
-  AWQ_REQUIRE(s.parts <= kMostParts && a.n_rows * s.parts < (1ll << 31), "too many logits");
+  AWQ_REQUIRE(s.parts <= kMostParts && launchable(a.n_rows * s.parts, kScan) && launchable(a.n_rows, kChoose), "too many logits");
   s.part = (Part*)a.workspace;
   s.histogram = (uint64_t*)(s.part + a.n_rows * s.parts);
   s.chunk = (float*)(s.histogram + a.n_rows * s.parts * kBins);

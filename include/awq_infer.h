@@ -690,7 +690,8 @@ int awq_polynorm(void* z, int64_t ld, int64_t n, int64_t n_tokens, const float* 
  * `dtype`: AWQ_DTYPE_BFLOAT16 or AWQ_DTYPE_FLOAT16 (awq_sample: or
  * AWQ_DTYPE_FLOAT32).  Device pointers on the current device; 16-bit
  * activations 16-byte aligned, their strides (in values) multiples of 8.  Nothing
- * is allocated and the host is not waited for, so that every call may be captured.
+ * is allocated and the host is not waited for, so that every call may be captured.  A call that would
+ * take a launch of 2^32 threads or more is refused.
  *
  * The cache is n_pages pages of 64 positions, [page][kv_head][72 * dim bytes],
  * dim 64, 128 or 256, 16-byte aligned.  A head's part of a page: its keys [64][dim / 2 bytes], its values
