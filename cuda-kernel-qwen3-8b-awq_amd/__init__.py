@@ -251,6 +251,7 @@ class AwqRotarySpec(ctypes.Structure):
 
 
 ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_BANDS = range(4)
+ROTARY_TURNS = 5
 SIGNATURES.update({
     "awq_page_bytes": (_i64, [_i32, _i32]),
     "awq_page_plan": (ctypes.c_int, [ctypes.POINTER(AwqPagePlanArgs), _vp]),

@@ -26,24 +26,26 @@ extern "C" int awq_page_plan(const awq_page_plan_args* a, void* stream) {
 
 extern "C" int awq_rotary_tables(const awq_rotary_spec* s, int64_t max_pos, float* cosines, float* sines) {
   AWQ_REQUIRE(s != nullptr && cosines && sines, "NULL pointer");
-  AWQ_REQUIRE(s->kind >= AWQ_ROTARY_PLAIN && s->kind <= AWQ_ROTARY_BANDS, "unknown kind");
+  const bool bands = s->kind == AWQ_ROTARY_BANDS || s->kind == AWQ_ROTARY_TURNS;
+  AWQ_REQUIRE(bands || (s->kind >= AWQ_ROTARY_PLAIN && s->kind <= AWQ_ROTARY_BASE), "unknown kind");
   AWQ_REQUIRE(s->rot >= 2 && s->rot % 2 == 0 && s->rot <= 65536 && max_pos >= 0, "rot or max_pos out of range");
   AWQ_REQUIRE(s->base > 1.0 && isfinite(s->base), "base must be above 1");
   AWQ_REQUIRE(s->kind == AWQ_ROTARY_PLAIN || (s->factor >= 1.0 && isfinite(s->factor)), "factor must be at least 1");
   AWQ_REQUIRE(s->kind != AWQ_ROTARY_BASE || s->rot > 2, "one pair alone has no lowest frequency to divide");
-  AWQ_REQUIRE(s->kind != AWQ_ROTARY_BANDS || (s->original > 0.0 && s->slow > 0.0 && s->fast > s->slow && isfinite(s->original) && isfinite(s->fast)),
+  AWQ_REQUIRE(!bands || (s->original > 0.0 && s->slow > 0.0 && s->fast > s->slow && isfinite(s->original) && isfinite(s->fast)),
               "bands need original > 0 and 0 < slow < fast");
   const int half = s->rot / 2;
   const double base = s->kind == AWQ_ROTARY_BASE ? s->base * pow(s->factor, (double)s->rot / (s->rot - 2)) : s->base;
-  const double amplitude = s->kind == AWQ_ROTARY_BANDS ? 0.1 * log(s->factor) + 1.0 : 1.0;
+  const double amplitude = bands ? 0.1 * log(s->factor) + 1.0 : 1.0;
   // the index at which a frequency makes `turns` turns in `original` positions: original base^(-2 i / rot) = 2 pi turns
   const auto index_of = [&](double turns) { return s->rot * log(s->original / (2.0 * M_PI * turns)) / (2.0 * log(s->base)); };
   for (int i = 0; i < half; ++i) {
     double f = pow(base, -2.0 * i / s->rot);
     if (s->kind == AWQ_ROTARY_LINEAR) f /= s->factor;
-    if (s->kind == AWQ_ROTARY_BANDS) {
-      const double first = index_of(s->fast), last = index_of(s->slow);
-      const double share = fmin(fmax((i - first) / (last - first), 0.0), 1.0);  // of the divided frequency
+    if (bands) {
+      const double first = index_of(s->fast), last = index_of(s->slow), turns = s->original * f / (2.0 * M_PI);
+      const double at = s->kind == AWQ_ROTARY_BANDS ? (i - first) / (last - first) : (s->fast - turns) / (s->fast - s->slow);
+      const double share = fmin(fmax(at, 0.0), 1.0);  // of the divided frequency
       f = f * (1.0 - share) + f / s->factor * share;
     }
     for (int64_t p = 0; p < max_pos; ++p) {

@@ -747,16 +747,19 @@ int awq_page_plan(const awq_page_plan_args* args, void* stream);
  *                      is divided by factor, the highest stays
  *   AWQ_ROTARY_BANDS   f_i / factor below `slow` turns in `original` positions, f_i
  *                      above `fast` turns, between them linearly from one to the other
- *                      in the index at which a frequency makes so many turns; amplitude 0.1 ln(factor) + 1
- *                      (the method of the YaRN paper, Peng et al. 2023) */
+ *                      in the index at which a frequency makes so many turns, which need not be a whole one (for
+ *                      bounds at whole indices b pass their turns, original base^(-2 b / rot) / 2 pi); amplitude 0.1 ln(factor) + 1
+ *   AWQ_ROTARY_TURNS   the same, but between them linearly in the number of turns itself, original base^(-2 i / rot) / 2 pi
+ *                      (the ramp of the YaRN paper, Peng et al. 2023; the two differ in most of the frequencies between) */
 #define AWQ_ROTARY_PLAIN 0
 #define AWQ_ROTARY_LINEAR 1
 #define AWQ_ROTARY_BASE 2
 #define AWQ_ROTARY_BANDS 3
+#define AWQ_ROTARY_TURNS 5 /* (4 is no kind) */
 typedef struct awq_rotary_spec {
   int32_t kind, rot;
   double base, factor;           /* factor >= 1 */
-  double original, slow, fast;   /* AWQ_ROTARY_BANDS */
+  double original, slow, fast;   /* AWQ_ROTARY_BANDS and AWQ_ROTARY_TURNS */
 } awq_rotary_spec;
 int awq_rotary_tables(const awq_rotary_spec* spec, int64_t max_pos, float* cosines, float* sines);
 
