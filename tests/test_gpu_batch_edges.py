@@ -153,6 +153,25 @@ def test_paged_attention_of_scales_below_zero(dev, dtype, heads, kv, dim, size, 
     check_paged(got.reshape(3, heads, dim), dtype, vq.reshape(3, heads, dim), table, lengths, k, v, spread, n_pages, dim ** -0.5)
 
 
+@pytest.mark.parametrize("dim,long", [(64, 2500), (256, 1250)])
+def test_paged_attention_of_many_pages_a_wavefront(dev, dim, long):
+    """128 key/value heads leave a wavefront more than 64 pages of one request: its page numbers are read anew while pages are on their way"""
+    kv, few = 128, [0, 77]
+    lengths = [200, 64 * long - 7, 1, 64 * 90]
+    rng = rng_of("many pages", dim)
+    print("paged, many pages", dim, flush=True)
+    n_pages, width = 9, long
+    cache, k, v, spread = cache_of(dev, rng, n_pages, kv, dim)
+    table = rng.integers(0, n_pages, (4, width))
+    table[rng.random(table.shape) < 0.1] = -1
+    table[1, 60:130] = np.where(np.arange(70) % 7 == 0, 3, -1)
+    x = rng.standard_normal((4, kv * dim))
+    d_q, vq = dev.act(x, "f16")
+    got = paged(dev, "f16", d_q, cache, table, lengths, kv, kv, dim, dim ** -0.5, dev.full((4, kv * dim), 9.0, "f16")).reshape(4, kv, dim)
+    k, v, spread = (t[:, few] for t in (k, v, spread))
+    check_paged(got[:, few], "f16", vq.reshape(4, kv, dim)[:, few], table, lengths, k, v, spread, n_pages, dim ** -0.5)
+
+
 # --- attention of packed prompts ----------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("dim", [64, 128, 256])
