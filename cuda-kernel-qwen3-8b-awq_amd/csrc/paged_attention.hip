@@ -11,7 +11,7 @@ typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;     // of a workgroup, each with pages of its own
 constexpr int kColumns = 16;  // query heads of one key/value head that share a pass over the pages
-constexpr float kSlack = 8.0f;
+constexpr float kSlack = 8.0f, kNone = -1000.0f;  // kNone: r of a group without any products yet
 
 // Wavefronts of a SIMD: as many as have all their numbers in registers.  Heads of 128, 64 requests of 8 key/value heads with 4 query heads each:
 // 4 (some numbers in scratch memory) 49 us, 3 42, 2 44; 2 key/value heads with 16: 4 37 us, 2 20; heads of 256 with 16: 2 39 us, 1 25.
@@ -82,9 +82,9 @@ __device__ __forceinline__ int run_of(int all, int workers) { return (all + work
 // sum over a group, s sum(q n) + z sum(q) in binary32, and on the weights, p s rounded to binary16 for the product, p z in binary32.
 // Heads of 128, 32 over 8: 64 requests of 100 to 8,000 positions, bfloat16, 42 us, 4.2 TB/s of the cache; one of 40,960 positions, binary16, 17 us (its
 // 640 pages leave a worker two); 12 requests of 5 to 300 positions, 16 heads of 64, 6 us.  Bound by memory and, at a few pages a worker, by the start.
-// Weights are relative to the largest score, rounded up to a whole number so that moving it is exact.  A group's products p s are relative to a power of
-// two of its own, 2^r times that, which moves once some are 2^kSlack above it: they are normal numbers of binary16 down to 2^-14 of the group's largest
-// so far, whatever the scales of keys that weigh nothing and of other groups, and whatever their sign.
+// Weights are relative to the largest score, whose own is 1 then and its products p s exact.  A group's products are held relative to a power of two of
+// its own, 2^r for a whole r, which moves once some are 2^kSlack above it: they are normal numbers of binary16 down to 2^-14 of the group's largest so
+// far, whatever the scales of keys that weigh nothing and of other groups, and whatever their sign.
 template <typename T, int D, int COLUMNS>
 __global__ __launch_bounds__(64 * kWaves, resident(D, COLUMNS)) void paged_kernel(PagedArgs p) {
   constexpr int G = D / 64, PIECES = D / 32;  // groups; 16-byte pieces of a row
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(64 * kWaves, resident(D, COLUMNS)) void paged_kerne
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       off[g] = 0.0f;
-      r2[g] = -INFINITY;
+      r2[g] = kNone;
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[g][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(64 * kWaves, resident(D, COLUMNS)) void paged_kerne
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the keys and the parameters have been read
       if (next >= 0) request_keys(next);
       highest = over_head<COLUMNS>(highest, lanes::Max());
-      const float to_best = fmaxf(best, __builtin_ceilf(highest));
+      const float to_best = fmaxf(best, highest);
       if (__builtin_amdgcn_ballot_w64(to_best > best)) {
         const float step = to_best > best ? to_best - best : 0.0f, alpha = __builtin_amdgcn_exp2f(-step);
         best = to_best;
@@ -326,7 +326,12 @@ __global__ __launch_bounds__(64 * kWaves, resident(D, COLUMNS)) void paged_kerne
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           off[g] *= alpha;
-          r2[g] -= step;  // (the sums of products stay as they are)
+          // (the group's largest so far are `step` less by now, and so is r as far as it stays whole)
+          const float r = r2[g] - step;
+          r2[g] = fmaxf(__builtin_ceilf(r), kNone);
+          const float rest = __builtin_amdgcn_exp2f(r - r2[g]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[g][j] *= rest;
         }
       }
       const float base = best == -INFINITY ? 0.0f : best;
@@ -356,7 +361,7 @@ __global__ __launch_bounds__(64 * kWaves, resident(D, COLUMNS)) void paged_kerne
 #pragma unroll
           for (int j = 0; j < 4; ++j) o[g][j] *= alpha;
         }
-        const float up = __builtin_amdgcn_exp2f(fminf(-r2[g], 126.0f));
+        const float up = __builtin_amdgcn_ldexpf(1.0f, (int)fminf(-r2[g], 126.0f));
 #pragma unroll
         for (int q = 0; q < SETS; ++q) {
           half4_t ps;
@@ -425,7 +430,7 @@ __global__ __launch_bounds__(64 * kWaves, resident(D, COLUMNS)) void paged_kerne
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       off[g] = over_head<COLUMNS>(off[g], lanes::Add());
-      const float size = __builtin_amdgcn_exp2f(r2[g]);
+      const float size = __builtin_amdgcn_ldexpf(1.0f, (int)r2[g]);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -450,7 +455,9 @@ __global__ __launch_bounds__(64 * kWaves, resident(D, COLUMNS)) void paged_kerne
       __syncthreads();
       whole = wg_begin == start && wg_end == start + n_pages;
       const int64_t slot = ((int64_t)stream * p.workers + worker - wave) * 2 + (start < wg_begin ? 0 : 1);
-      for (int x = threadIdx.x; x < columns * (D / 4); x += 64 * kWaves) {
+      int tid = threadIdx.x;
+      if constexpr (D == 256) asm volatile("" : "+v"(tid));  // (as below)
+      for (int x = tid; x < columns * (D / 4); x += 64 * kWaves) {
         const int c = x / (D / 4), d = x % (D / 4) * 4;
         float top = -INFINITY, total = 0.0f;
 #pragma unroll

@@ -153,6 +153,28 @@ def test_paged_attention_of_scales_below_zero(dev, dtype, heads, kv, dim, size, 
     check_paged(got.reshape(3, heads, dim), dtype, vq.reshape(3, heads, dim), table, lengths, k, v, spread, n_pages, dim ** -0.5)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (12, 2, 128), (16, 1, 128), (8, 2, 256), (16, 1, 256)])
+@pytest.mark.parametrize("position", [0, 70])
+def test_paged_attention_of_one_key_is_its_value(dev, dtype, heads, kv, dim, position):
+    """where one key has all the weight its product with the scale is exact: the value is rounded once, behind sums in binary32"""
+    rng = rng_of("one key", dtype, heads, dim, position)
+    n, L = 40, position + 1
+    table, n_pages = tables(rng, n, [plain.pages(L)] * n, 2)
+    cache, k, v, spread = cache_of(dev, rng, n_pages, kv, dim)
+    q = np.ones((n, heads * dim))
+    if position:  # all other keys have none: theirs are far below
+        raw = cache.view(dev.torch.float16).reshape(n_pages, kv, 36 * dim)[:, :, 32 * dim:34 * dim].reshape(n_pages, kv, dim // 64, 2, 64)
+        raw[:, :, :, 0], raw[:, :, :, 1] = 0.0, -60000.0
+        raw[:, :, :, 1, position % 64].fill_(100.0)
+        raw[dev.torch.from_numpy(table[:, 0]).cuda(), :, :, 1] = -60000.0
+    d_q, _ = dev.act(q, dtype)
+    got = paged(dev, dtype, d_q, cache, table, [L] * n, heads, kv, dim, dim ** -0.5, dev.full((n, heads * dim), 9.0, dtype)).reshape(n, heads, dim)
+    of = table[:, position // 64], slice(None), position % 64
+    want, size = (np.repeat(t[of], heads // kv, 1) for t in (v, spread))
+    assert (np.abs(got - want) <= plain.EPS[dtype] / 2 * np.abs(want) + 2.0 ** -21 * size + (2.0 ** -25 if dtype == "f16" else 0.0)).all()
+
+
 @pytest.mark.parametrize("dim,long", [(64, 2500), (256, 1250)])
 def test_paged_attention_of_many_pages_a_wavefront(dev, dim, long):
     """128 key/value heads leave a wavefront more than 64 pages of one request: its page numbers are read anew while pages are on their way"""
