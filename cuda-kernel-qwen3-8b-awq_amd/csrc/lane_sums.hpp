@@ -38,6 +38,15 @@ __device__ __forceinline__ float over(float v, F f) {
   }
   return v;
 }
+// over the lanes 16 apart, in every lane
+template <typename F>
+__device__ __forceinline__ float over_rows(float v, F f) {
+  float a = v, b = v;
+  asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+  a = b = f(a, b);
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+  return f(a, b);
+}
 template <int N = 64>
 __device__ __forceinline__ float sum(float v) {
   return over<N>(v, Add());

@@ -44,8 +44,7 @@ template <int FROM, typename F>
 __device__ __forceinline__ float over_head(float v, F f) {
   if constexpr (FROM <= 4) v = f(v, lanes::from<0x124>(v));  // rotated by 4 within 16 lanes, and by 8
   if constexpr (FROM <= 8) v = f(v, lanes::from<0x128>(v));
-  v = f(v, __shfl_xor(v, 16, 64));
-  return f(v, __shfl_xor(v, 32, 64));
+  return lanes::over_rows(v, f);
 }
 
 __device__ __forceinline__ int pages_of(const awq_paged_attention_args& a, int r) {
