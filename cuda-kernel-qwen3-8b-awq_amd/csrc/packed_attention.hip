@@ -26,7 +26,8 @@ constexpr int kQueries = 128;
 
 // The tile of queries a workgroup takes: request r has ceil(queries / 128) of them.  Every wavefront looks its own up.  False: there are fewer tiles.
 // Up to 64 requests, a lane each: tiles with the most keys first, by 128 keys; what runs last is short.  (13 prompts of 60 to 1,000 tokens, one request
-// behind the other 50 us, so 47; 3 parts of long prompts, all long, 188 and 189.)  More requests: one behind the other, 64 at a time, the last tile of each first, which has
+// behind the other 50 us, so 47; 3 parts of long prompts, all long, 188 and 189; next to the border no gain, 32 prompts of 20 to 600 tokens 98 and 96,
+// 64 of them 178 and 183.)  More requests: one behind the other, 64 at a time, the last tile of each first, which has
 // the most keys; the search would read them all some ten times.
 struct Tile {
   int q_begin, q_end, k_begin, k_end, first;  // first: of the tile's queries, from q_begin on
@@ -114,8 +115,8 @@ __device__ __forceinline__ u32x4_t only_finite(u32x4_t v) {
 // A step's scores are formed during the step ahead, each product of theirs beside a few of its weights, so that matrix and vector instructions of one
 // wavefront run together; keys are therefore requested two steps ahead, values one.  (What is on its way is waited for ahead of a step's first
 // transposing read, the compiler's doing, and ahead of the next barrier: a request runs beside the step's masks and maximum.)
-// Heads of 128, 32 over 8: 13 prompts of 60 to 1,000 tokens, binary16, 46 us; 3 parts of 500 to 1,100 tokens behind 3,500 each, bfloat16, 179 us, 0.74 PFLOP/s.
-// Bound by the two kinds of instructions (each a third of the time) and by 800 workgroups on 512 places.  64 keys a step and two wavefronts a
+// Heads of 128, 32 over 8: 13 prompts of 60 to 1,000 tokens, binary16, 42 us a call in a row, 46 traced; 3 parts of 500 to 1,100 tokens behind 3,500 each,
+// bfloat16, 168 us, 0.79 PFLOP/s, and 205.  (The other figures here are traced ones of their time, against each other.)  Bound by the two kinds of instructions (each a third of the time) and by 800 workgroups on 512 places.  64 keys a step and two wavefronts a
 // SIMD: 32 keys and three 57 and 236 us where these took 54 and 216; scores in their own step 53 and 206, formed a step ahead 50 and 188 (and 47 and 179 with the first values
 // read ahead of them); heads of 64 with three wavefronts, some numbers in scratch memory, 74 us, with two 72.
 // Where some query of the workgroup does not see all keys of a step, values that are not finite are kept out of the product, in which 0 times

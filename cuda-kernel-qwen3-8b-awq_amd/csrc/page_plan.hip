@@ -57,7 +57,7 @@ __device__ __forceinline__ void write_slot(const awq_page_plan_args& a, int64_t 
 // One workgroup, 1,024 requests at a time: pages given back, then pages taken, each by a thread a page that looks its request up
 // among the sums in LDS.  SLOTS: the new positions' slots too, where one workgroup has all requests in LDS and few
 // positions a thread; slots_kernel otherwise.
-// Bound by its trips to memory and barriers one behind the other, not by bytes: 200 answers 9 us.
+// Bound by its trips to memory and barriers one behind the other, not by bytes: 200 answers, five of them ended, 9.8 us (traced).
 template <bool SLOTS>
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(awq_page_plan_args a) {
   __shared__ int part[48], sums[kPlanThreads], held_of[kPlanThreads], length_of[kPlanThreads], cached_of[kPlanThreads];
@@ -182,7 +182,8 @@ __global__ __launch_bounds__(kSlotThreads) void slots_kernel(awq_page_plan_args 
 
 }  // namespace
 
-// One launch or two: 200 requests with a position each 9.0 us in one, 8.1 + 2.1 in two; 240 requests with 10,800 positions 17.1 us in one, 8.3 + 3.5 in two.
+// One launch or two (traced, none ended): 200 requests with a position each 7.6 us in one, 6.6 + 2.5 in two; next to the border 1,000 requests with 4,000
+// positions 10.9 and 8.0 + 4.1, 240 with 4,080 10.2 and 6.8 + 4.2; behind it 240 with 10,800 17.1 and 8.3 + 3.5.
 int launch_page_plan(const awq_page_plan_args& a, hipStream_t st) {
   if (a.n_requests <= kPlanThreads && a.max_tokens <= kPlanTokens) {
     hipLaunchKernelGGL(plan_kernel<true>, dim3(1), dim3(kPlanThreads), 0, st, a);

@@ -80,7 +80,7 @@ __device__ __forceinline__ int run_of(int all, int workers) { return (all + work
 // so are the sums of the values' pieces), so that a word of eight takes five instructions.  The scales are put on afterwards: on a key's
 // sum over a group, s sum(q n) + z sum(q) in binary32, and on the weights, p s rounded to binary16 for the product, p z in binary32.
 // Heads of 128, 32 over 8: 64 requests of 100 to 8,000 positions, bfloat16, 42 us, 4.2 TB/s of the cache; one of 40,960 positions, binary16, 17 us (its
-// 640 pages leave a worker two); 12 requests of 5 to 300 positions, 16 heads of 64, 6 us.  Bound by memory and, at a few pages a worker, by the start.
+// 640 pages leave a worker two); 12 requests of 5 to 300 positions, 16 heads of 64, 6 us (all traced).  Bound by memory and, at a few pages a worker, by the start.
 // Weights are relative to the largest score, whose own is 1 then and its products p s exact.  A group's products are held relative to a power of two of
 // its own, 2^r for a whole r, which moves once some are 2^kSlack above it: they are normal numbers of binary16 down to 2^-14 of the group's largest so
 // far, whatever the scales of keys that weigh nothing and of other groups, and whatever their sign.
@@ -594,7 +594,8 @@ void launch_pages(const PagedArgs& p, dim3 grid, hipStream_t st) {
 }
 
 // wide pieces of a request's values where the workers are cut over many requests, few parts each; narrow ones, whose threads share the parts,
-// where they are cut over few (one request of 40,960 positions 5.5 us with 32 pieces, 7.2 with 128; 64 requests 17.8 and 9.2)
+// where they are cut over few (one request of 40,960 positions 5.5 us with 32 pieces, 7.2 with 128; 64 requests 17.8 and 9.2; next to the border 5 requests
+// of 8,000 with 32 pieces and 6 with 128 take 4.8 and 4.7)
 int quads_of(const PagedArgs& p) { return p.workers / kWaves > 16ll * p.a.n_requests ? 32 : 128; }
 int chunks_of(const PagedArgs& p) { return (p.columns * p.a.dim + 4 * quads_of(p) - 1) / (4 * quads_of(p)); }
 

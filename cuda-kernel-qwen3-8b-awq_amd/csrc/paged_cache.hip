@@ -46,7 +46,7 @@ constexpr float kHalfMax = 65504.0f;
 // A thread takes eight values of a head of a token, so that 64 values with one scale are eight lanes side by side and a head is within
 // a wavefront.  Everything behind the load is in 64 bits, in which the turned values are exact: a value next to a border of the
 // number format, and a quotient next to a half, then go where the formula sends them.
-// 8,000 positions of 32 + 8 heads of 128, 64 of them turned, bfloat16: 55 us, 3.5 TB/s of what it reads and writes (190 MB), beside vector
+// 8,000 positions of 32 + 8 heads of 128, 64 of them turned, bfloat16: 56 us traced, 3.4 TB/s of what it reads and writes (190 MB), beside vector
 // instructions for most of that time.  64 positions: 4 us, a launch.
 template <typename T>
 __global__ __launch_bounds__(256) void append_kernel(awq_paged_append_args a, int blocks) {
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256) void append_kernel(awq_paged_append_args a, in
 constexpr int kRowsStarts = 4096;
 
 // A thread takes eight values of a row of keys or values; the request of a row is looked up among the starts.
-// 8,000 rows of 8 heads of 128, bfloat16: 22 us for 42 MB; bound by its 350 instructions a thread, 100 of them for eight roundings that are one each
+// 8,000 rows of 8 heads of 128, bfloat16: 22 us traced, 17 in a row, for 42 MB; bound by its 350 instructions a thread, 100 of them for eight roundings that are one each
 // (the requests' numbers in LDS for two trips to memory fewer: no gain).
 template <typename T>
 __global__ __launch_bounds__(256) void rows_kernel(awq_paged_rows_args a) {

@@ -9,7 +9,7 @@ namespace {
 // between e^(-1/8) and 1, as a whole multiple of 2^-36, so that sums do not depend on their order; bins are joined in 64-bit floating point.
 // (Tokens with the largest logit are all in the first bin: their sums are exact, and uniform numbers such as 1/2 fall between two of them as
 // they should.)
-// 151,936 logits a row.  256 rows of binary32: scan 50 us filtered, 46 not, 29 greedy (33 us of a copy's rate; LDS additions and 64-bit arithmetic),
+// 151,936 logits a row, traced.  256 rows of binary32: scan 50 us filtered, 46 not, 29 greedy (33 us of a copy's rate; LDS additions and 64-bit arithmetic),
 // choose 18 us for top-k 50, 44 to 64 for top-p (a bin of thousands, whose tokens are in most chunks: one compute unit reads the row again).  One row of binary16: 6 us,
 // and 6 unfiltered, 15 top-k, 28 to 39 top-p: bound by steps one behind the other, of a trip to memory or a barrier each.
 //   scan_kernel    parts of 8,192 logits: largest, sum of weights, and where a row is filtered a histogram, sums and counts by bin

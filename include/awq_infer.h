@@ -809,7 +809,9 @@ int awq_paged_rows(const awq_paged_rows_args* args, int32_t dtype, void* stream)
 /* Attention of one query a request over the first lengths[i] positions of its pages
  * (up to 64 max_pages): row i of q and ctx, head h on key/value head h / (heads / kv_heads),
  * softmax of scale q . k, weighted sum of v.  No position: zeros.  The work is cut evenly over the chip whatever the lengths; the cut, and
- * with it the order of a request's sums, depends on all lengths of the call.  workspace:
+ * with it the order of a request's sums, depends on all lengths of the call.  Scores, sums and maxima are
+ * binary32; a query's values go into the products as binary16 numbers times a power of two of its own, and a weight times
+ * its value's scale is rounded to binary16 relative to the largest of its group of 64.  workspace:
  * awq_paged_workspace_bytes, 16-byte aligned, contents irrelevant; calls that share one must not overlap. */
 typedef struct awq_paged_attention_args {
   const void* q;
@@ -830,7 +832,7 @@ int awq_paged_attention(const awq_paged_attention_args* args, int32_t dtype, voi
  * q_starts[i] .. q_starts[i + 1] - 1 and the keys k_starts[i] .. k_starts[i + 1] - 1 (k_starts NULL: as
  * q_starts), both ascending, on the device.  causal != 0: the last query sees all keys and
  * each query ahead of it one fewer; 0: all see all.  A query without keys: zeros.  Rows of ctx that belong to no request stay as they
- * were.  n_tokens, n_keys: rows of q and of k and v; those of k and v are at most 2^25 values apart. */
+ * were.  Scores, sums and maxima are binary32; a weight is rounded to dtype for its product with v.  n_tokens, n_keys: rows of q and of k and v; those of k and v are at most 2^25 values apart. */
 typedef struct awq_packed_attention_args {
   const void* q;
   const void* k;
@@ -853,7 +855,7 @@ int awq_packed_attention(const awq_packed_attention_args* args, int32_t dtype, v
  * the first always.  ids[row] = the first kept id, in rising order, at which the sum of the weights kept exceeds uniform[row]
  * (in [0, 1)) times all of it.  T not above 0 (or NaN): the first token.  A NaN logit counts as -infinity; logits of +infinity share all the weight;
  * a row without a logit above -infinity: 0.  temperature NULL: 1; top_k, top_p, min_p NULL (or an entry of top_p or min_p NaN): not limited.
- * Weights and sums are held in 64 bits.  workspace: awq_sample_workspace_bytes, 16-byte aligned, contents irrelevant; calls that share one must not overlap. */
+ * A weight is good to some 1e-11 of it plus 2^-52 |l| / T; sums of weights are whole numbers and 64-bit ones, in one order.  workspace: awq_sample_workspace_bytes, 16-byte aligned, contents irrelevant; calls that share one must not overlap. */
 typedef struct awq_sample_args {
   const void* logits;
   const float* temperature;
