@@ -712,7 +712,7 @@ int64_t awq_page_bytes(int32_t kv_heads, int32_t dim);
 
 /* Pages and slots of the next positions of n_requests requests (n_requests (64 max_pages + 1) and 64 n_pages below 2^31).
  * Request i has cached[i] positions (0 .. 64 max_pages) and gets fresh[i] more (up to 64 max_pages); fresh[i] < 0: it
- * has ended and its pages go back.  free_pages [n_pages] with *free_in entries is a
+ * has ended and its pages go back.  free_pages [n_pages] with *free_in entries, each a page that nobody has, is a
  * list from whose end pages are taken: first the pages of ended requests are put
  * on it in the order of the requests (entries of theirs that are no pages are passed over), then the requests take theirs in order.  A request that does not fit in max_pages is
  * left out; one that needs pages is left out too where all that the requests up to it need together is
